@@ -333,6 +333,89 @@ RLA_API size_t rla_w8a16_swiglu_workspace_size(int64_t M, int64_t N, int64_t K);
 RLA_API int rla_rmsnorm(const void* x, int64_t ldx, const void* weight, int weight_dtype, float eps, void* y,
                         int64_t ldy, int64_t M, int64_t K, void* stream);
 
+/*
+ * RMSNorm with the residual's addition, rows of length K (no counterpart in
+ * rotalabs-accel, whose rmsnorm (src/rotalabs_accel/kernels/normalization.py:186-213)
+ * takes one tensor; this is the same norm where a decoder layer uses it):
+ *
+ *     h = T(x + residual)                     (h = x where residual is NULL)
+ *     v = h * rsqrt(mean(h^2) + eps) * weight (fp32)
+ *     rla_add_rmsnorm:       y = T(v)
+ *     rla_add_rmsnorm_int8:  scale[m] = max|v| / 127 (1 for a zero row),
+ *                            q = rint(v / scale[m])
+ *
+ * T is `dtype` (F16 or BF16), the type of x, residual, h and y; weight [K] is
+ * F32, F16 or BF16.  Row strides are in elements, any alignment (rows that
+ * are 16-byte aligned run fastest).  h is written only where residual is
+ * given and must not overlap x or residual.  An int8 row whose v holds an
+ * infinity or NaN gets the scale NaN and q = 0.  K <= 2^30.
+ */
+RLA_API int rla_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype,
+                            const void* weight, int weight_dtype, float eps, void* h, int64_t ldh, void* y,
+                            int64_t ldy, int64_t M, int64_t K, void* stream);
+RLA_API int rla_add_rmsnorm_int8(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype,
+                                 const void* weight, int weight_dtype, float eps, void* h, int64_t ldh, int8_t* q,
+                                 int64_t ldq, float* scale, int64_t M, int64_t K, void* stream);
+
+/*
+ * SwiGLU with an 8-bit output: v = silu(gate) * up in fp32, then scale and q
+ * of each row as in rla_add_rmsnorm_int8.  gate and up are [M, N] of `dtype`
+ * (F16 or BF16).  The activation of rotalabs-accel's swiglu_fused
+ * (src/rotalabs_accel/kernels/activations.py:109-137) where an 8-bit down
+ * product follows.
+ */
+RLA_API int rla_swiglu_int8(const void* gate, int64_t ldg, const void* up, int64_t ldu, int dtype, int8_t* q,
+                            int64_t ldq, float* scale, int64_t M, int64_t N, void* stream);
+
+/*
+ * W8A8 product: int8 rows with one fp32 scale each times int8 weights with
+ * one scale an output channel,
+ *
+ *     y[m, n] = fp16( x_scale[m] * scale[n] * sum_k x[m, k] * w[n, k]  (+ bias[n]) ),
+ *
+ * the sum exact in int32 (so K < 131072, else RLA_ERR_UNSUPPORTED).  x
+ * [M, K] and w [N, K] with any row stride and alignment; rows that are not
+ * 16-byte aligned (pointer, or stride of more than one row) are first copied
+ * into `workspace` (16-byte aligned, rla_w8a8_workspace_size bytes suffice;
+ * may be NULL where both operands are aligned).  No counterpart in
+ * rotalabs-accel, which quantizes weights only.
+ */
+RLA_API int rla_w8a8_gemm(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+                          const void* scale, int scale_dtype, const void* bias, int bias_dtype, void* y, int64_t ldy,
+                          int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+RLA_API size_t rla_w8a8_workspace_size(int64_t M, int64_t N, int64_t K);
+
+/*
+ * A whole mixture-of-experts layer for a few tokens, with int8 expert weights
+ * (no counterpart in rotalabs-accel; each expert is its SwiGLU block,
+ * src/rotalabs_accel/kernels/activations.py:140-181, with W8A16 projections):
+ *
+ *     p = softmax(x router^T);  the top_k largest of each token, ties to the
+ *     lower index;  c = p, or p / (sum of the chosen p) with renormalize
+ *     a = fp16( silu(scale_gate * (w_gate x)) * (scale_up * (w_up x)) )   per chosen expert
+ *     y = fp16( sum over the chosen experts of c * scale_down * (w_down a) )
+ *
+ *   x       fp16 [T, H], row stride ldx; y fp16 [T, H], row stride ldy
+ *   router  fp16 [E, H]
+ *   w_gate, w_up int8 [E, I, H]; w_down int8 [E, H, I]; all contiguous
+ *   scales  [E, I], [E, I], [E, H] of scale_dtype (F32 or F16)
+ *   workspace  rla_moe_workspace_size(T, I, top_k) bytes, 256-byte aligned,
+ *           not shared by calls that may overlap
+ *
+ * Needs T <= RLA_MOE_MAX_TOKENS, E <= RLA_MOE_MAX_EXPERTS, top_k <=
+ * RLA_MOE_MAX_TOP_K, H and I multiples of 16, 16-byte aligned x rows, router
+ * and weights (else RLA_ERR_UNSUPPORTED).  Two kernels, no atomics on global
+ * memory, bit-reproducible.  A token whose logits hold NaN gets NaN.
+ */
+#define RLA_MOE_MAX_TOKENS 32
+#define RLA_MOE_MAX_EXPERTS 256
+#define RLA_MOE_MAX_TOP_K 32
+RLA_API int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate, const void* scale_gate,
+                    const int8_t* w_up, const void* scale_up, const int8_t* w_down, const void* scale_down,
+                    int scale_dtype, int renormalize, void* y, int64_t ldy, int64_t T, int64_t H, int64_t I, int64_t E,
+                    int64_t top_k, void* workspace, size_t workspace_bytes, void* stream);
+RLA_API size_t rla_moe_workspace_size(int64_t T, int64_t I, int64_t top_k);
+
 /* Number of kernels this library has launched in this process (all devices). */
 RLA_API uint64_t rla_launch_count(void);
 

@@ -39,6 +39,8 @@ EXPORTED_SYMBOLS = (
     "rla_peer_free", "rla_ipc_export", "rla_ipc_open", "rla_ipc_close",
     "rla_w8a16_gemm_swiglu", "rla_w8a16_swiglu_workspace_size", "rla_rmsnorm",
     "rla_w8a16_allgather_workspace_size", "rla_prefill_exchange_begin", "rla_prefill_exchange_block",
+    "rla_add_rmsnorm", "rla_add_rmsnorm_int8", "rla_swiglu_int8", "rla_w8a8_gemm", "rla_w8a8_workspace_size",
+    "rla_moe", "rla_moe_workspace_size",
 )
 
 MAX_PEERS = 8
@@ -53,6 +55,7 @@ _lib = None
 _fast = None
 _torch_op = None          # torch.ops.rla.w8a16_gemm.default (through the dispatcher)
 _torch_op_direct = None   # the same CUDA kernel function, called without the dispatcher
+_torch_ops = None         # the extension module itself
 _lib_lock = threading.Lock()
 
 
@@ -125,6 +128,24 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.rla_prefill_exchange_block.argtypes = [p, i64, p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                    i64, i64, i64, p, i64, p]
         lib.rla_prefill_exchange_block.restype = ctypes.c_int
+        lib.rla_add_rmsnorm.argtypes = [p, i64, p, i64, ctypes.c_int, p, ctypes.c_int, ctypes.c_float, p, i64, p, i64,
+                                        i64, i64, p]
+        lib.rla_add_rmsnorm.restype = ctypes.c_int
+        lib.rla_add_rmsnorm_int8.argtypes = [p, i64, p, i64, ctypes.c_int, p, ctypes.c_int, ctypes.c_float, p, i64, p,
+                                             i64, p, i64, i64, p]
+        lib.rla_add_rmsnorm_int8.restype = ctypes.c_int
+        lib.rla_swiglu_int8.argtypes = [p, i64, p, i64, ctypes.c_int, p, i64, p, i64, i64, p]
+        lib.rla_swiglu_int8.restype = ctypes.c_int
+        lib.rla_w8a8_gemm.argtypes = [p, i64, p, p, i64, p, ctypes.c_int, p, ctypes.c_int, p, i64, i64, i64, i64, p, sz,
+                                      p]
+        lib.rla_w8a8_gemm.restype = ctypes.c_int
+        lib.rla_w8a8_workspace_size.argtypes = [i64, i64, i64]
+        lib.rla_w8a8_workspace_size.restype = sz
+        lib.rla_moe.argtypes = [p, i64, p, p, p, p, p, p, p, ctypes.c_int, ctypes.c_int, p, i64, i64, i64, i64, i64,
+                                i64, p, sz, p]
+        lib.rla_moe.restype = ctypes.c_int
+        lib.rla_moe_workspace_size.argtypes = [i64, i64, i64]
+        lib.rla_moe_workspace_size.restype = sz
         if os.path.abspath(path) == LIB_PATH:
             # linked to this library by soname: the loader reuses the copy
             # loaded above, so both bindings share one library state
@@ -139,6 +160,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                     # static registration defines torch.ops.rla.w8a16_gemm
                     from . import _rla_torch_ops
                     globals()["_torch_op_direct"] = _rla_torch_ops.w8a16_gemm
+                    globals()["_torch_ops"] = _rla_torch_ops
                     globals()["_torch_op"] = torch.ops.rla.w8a16_gemm.default
                 except (ImportError, OSError, RuntimeError, AttributeError):
                     pass
@@ -413,6 +435,18 @@ def ipc_open(handle: bytes) -> int:
 
 def ipc_close(ptr: int) -> None:
     _check(load_library().rla_ipc_close(ptr), "rla_ipc_close")
+
+
+def torch_ops():
+    """The ``_rla_torch_ops`` extension module (the CUDA functions of the
+    8-bit activation path and the mixture-of-experts layer)."""
+    if _torch_ops is None:
+        load_library()
+        if _torch_ops is None:
+            raise RuntimeError(
+                f"rotalabs_accel_b200: {TORCH_OP_PATH} is missing or does not load; build it with "
+                "`python -m rotalabs_accel_b200.build` (there is no non-CUDA path for CUDA tensors)")
+    return _torch_ops
 
 
 _sm_counts: dict = {}

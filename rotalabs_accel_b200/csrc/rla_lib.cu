@@ -8,3 +8,6 @@
 #include "rla_noalloc.cu"
 #include "rla_peer.cu"
 #include "rla_xchg.cu"
+#include "rla_rows.cu"
+#include "rla_w8a8.cu"
+#include "rla_moe.cu"

@@ -28,6 +28,7 @@ import torch
 
 from . import _capi
 from .gemm import Int8Linear, _as_2d_fp16, int8_gemm
+from .w8a8 import int8_gemm_w8a8, swiglu_int8
 
 
 def rmsnorm_torch(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -146,6 +147,18 @@ class Int8SwiGLU(torch.nn.Module):
         h = int8_gemm_swiglu(x, self.w_gate.weight_int8, self.w_gate.scale, self.w_up.weight_int8, self.w_up.scale,
                              self.w_gate.bias, self.w_up.bias)
         return self.w_down(h)
+
+    def forward_w8a8(self, x_int8: torch.Tensor, x_scale: torch.Tensor) -> torch.Tensor:
+        """The block on int8 activations (``add_rmsnorm_int8``'s ``q`` and
+        ``scale``): gate and up by ``int8_gemm_w8a8``, ``swiglu_int8``, down by
+        ``int8_gemm_w8a8``.  Returns fp16 ``(..., hidden)``."""
+        for lin in (self.w_gate, self.w_up, self.w_down):
+            if not lin._quantized:
+                raise RuntimeError("Weights not quantized. Call quantize_weights() first.")
+        gate = int8_gemm_w8a8(x_int8, x_scale, self.w_gate.weight_int8, self.w_gate.scale, self.w_gate.bias)
+        up = int8_gemm_w8a8(x_int8, x_scale, self.w_up.weight_int8, self.w_up.scale, self.w_up.bias)
+        q, s = swiglu_int8(gate, up)
+        return int8_gemm_w8a8(q, s, self.w_down.weight_int8, self.w_down.scale, self.w_down.bias)
 
     def extra_repr(self) -> str:
         return f"hidden_size={self.hidden_size}, intermediate_size={self.intermediate_size}"
