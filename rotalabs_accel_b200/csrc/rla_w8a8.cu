@@ -6,16 +6,23 @@
 // so K < 2^17), whatever order it is taken in: results do not depend on the
 // tile, the split of K or the number of CTAs.
 //
-// Orientation: a tile is 128 output channels (the MMA's M, the 128 TMEM
-// lanes) x BT tokens (the MMA's N), so the channel's scale and bias are two
-// registers of an epilogue thread, and one token costs BT = 16 columns, not
-// 128 rows.
+// Orientation: a tile is 128 (or, of a CTA pair, 256) output channels (the
+// MMA's M, the TMEM lanes) x up to 256 tokens (the MMA's N), so the channel's
+// scale and bias are two registers of an epilogue thread, and one token costs
+// 16 columns, not 128 rows.
 //
-// Work split.  The K axis of a tile is split over the CTAs of a thread-block
-// cluster where there are fewer tiles than SMs: every rank leaves its int32
-// partial tile in shared memory, and each rank adds up every splits-th token
-// column from all ranks through distributed shared memory.  No workspace, no
-// atomics.
+// Two kernels:
+//   split  one tile a cluster.  Where there are fewer tiles than SMs, the K
+//          axis is split over the CTAs of the cluster: every rank leaves its
+//          int32 partial tile in shared memory, and each rank adds up every
+//          splits-th token column from all ranks through distributed shared
+//          memory.  No workspace, no atomics.
+//   pair   persistent CTA pairs (cta_group::2), 256 x 256 tiles, for problems
+//          of many tiles.  Each CTA of a pair loads 128 channels and 128
+//          tokens of a k block and the MMA reads both CTAs' shared memory, so
+//          an SM takes 32 KB from L2 for each 512 clocks of MMA; a 128 x 256
+//          tile of one CTA would take 48 KB, more than L2 gives an SM.  Two
+//          accumulators: the epilogue of a tile runs under the next tile's MMAs.
 //
 // Warp roles (192 threads): warp 0 TMA producer (a ring of 128-byte-wide k
 // blocks, 128-byte swizzle), warp 1 TMEM allocation and MMA issue, warps 2-5
@@ -36,6 +43,8 @@ constexpr int MAX_STAGES = 12;
 constexpr int MAX_SPLITS = 8;  // portable cluster size
 constexpr int MAX_K = 131071;  // K * 128 * 128 < 2^31
 __host__ __device__ constexpr int stage_bytes(int bt) { return (BR + bt) * BK; }
+constexpr int PAIR_ROWS = 256;   // tile of a CTA pair: channels, and tokens
+constexpr int PAIR_STAGES = 6;   // 32 KB each
 }  // namespace w8
 
 // D[tmem] (+)= A[smem] * B[smem]^T, kind::i8 (signed 8-bit inputs, int32 accumulate).
@@ -61,11 +70,86 @@ RLA_DEVFN void rla_tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&v)[16]) {
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
 }
-RLA_DEVFN uint32_t rla_ld_dsmem_u32(uint32_t addr, uint32_t rank) {
-  uint32_t remote, v;
+RLA_DEVFN uint32_t rla_mapa(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return remote;
+}
+RLA_DEVFN int4 rla_ld_cluster_int4(uint32_t remote) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(remote)
+               : "memory");
   return v;
+}
+
+// ---- CTA pairs (cta_group::2): the even CTA of the cluster leads ----
+RLA_DEVFN void rla_umma2_ss_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this offset in both CTAs once the MMAs issued so far are done.
+RLA_DEVFN void rla_umma2_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          rla_smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+RLA_DEVFN void rla_tmem2_alloc(uint32_t* smem_result, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(rla_smem_u32(smem_result)),
+               "r"(ncols)
+               : "memory");
+}
+RLA_DEVFN void rla_tmem2_relinquish() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+RLA_DEVFN void rla_tmem2_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Tile copy into this CTA's shared memory that counts on a barrier of either CTA of the pair.
+RLA_DEVFN void rla_tma2_load_2d(void* smem_dst, const void* desc, uint32_t bar, int32_t c0, int32_t c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(rla_smem_u32(smem_dst)),
+      "l"(desc), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+RLA_DEVFN void rla_mbar_arrive_cluster(uint32_t remote) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+RLA_DEVFN bool rla_mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(rla_smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// rla_mbar_wait for a barrier that the other CTA of the pair arrives on too.
+RLA_DEVFN bool rla_mbar_wait_cluster(uint64_t* bar, uint32_t parity, unsigned int err, volatile int* abort_flag) {
+  if (rla_mbar_try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = rla_globaltimer();
+  uint32_t spins = 0;
+  while (true) {
+    if (rla_mbar_try_wait_cluster(bar, parity)) return true;
+    if ((++spins & 15u) == 0) {
+      if (abort_flag && *abort_flag) return false;
+      if (rla_globaltimer() - t0 > RLA_WAIT_LIMIT_NS) {
+        rla_record_error(err);
+        if (abort_flag) *abort_flag = 1;
+        return false;
+      }
+    }
+  }
 }
 
 struct W8Out {
@@ -79,32 +163,37 @@ struct W8Out {
   int M, N;
 };
 
-template <int BT>
+RLA_DEVFN float w8a8_channel(const void* p, int kind, int n) {  // kind: 0 none, 1 fp16, 2 fp32
+  return kind == 0 ? 0.f : kind == 1 ? __half2float(static_cast<const __half*>(p)[n]) : static_cast<const float*>(p)[n];
+}
+RLA_DEVFN __half w8a8_value(int sum, float sw, float sx, float bias) {
+  return __float2half_rn(fmaf(static_cast<float>(sum) * sw, sx, bias));
+}
+
+// bt: token columns of a tile, a multiple of 16 up to 256.
 __global__ void __launch_bounds__(w8::THREADS)
     w8a8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                      const W8Out out, int num_kb, int stages) {
-  constexpr int COLS = BT < 32 ? 32 : BT;  // TMEM columns (a power of two, at least 32)
-  constexpr int LD = BT < 32 ? 16 : 32;    // token columns of one TMEM load
-  constexpr uint32_t STAGE = w8::stage_bytes(BT);
+                      const W8Out out, int num_kb, int stages, int bt, int tmem_cols) {
+  const uint32_t stage = w8::stage_bytes(bt);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[w8::MAX_STAGES], empty[w8::MAX_STAGES], dfull;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_word;
-  __shared__ float sx_s[BT];
+  __shared__ float sx_s[256];
+  __shared__ __align__(16) float sw_s[w8::BR], bias_s[w8::BR];
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * w8::BR;
-  const int m0 = blockIdx.y * BT;
+  const int m0 = blockIdx.y * bt;
   const int splits = gridDim.z;
   const int rank = blockIdx.z;  // == cluster rank: the cluster spans z
   const int kb0 = static_cast<int>((int64_t)num_kb * rank / splits);
   const int nkb = static_cast<int>((int64_t)num_kb * (rank + 1) / splits) - kb0;
   volatile int* abort_flag = &abort_word;
 
-  rla_griddep_launch_dependents();
   if (threadIdx.x == 0) {
     rla_tma_prefetch_desc(&tmap_w);
     rla_tma_prefetch_desc(&tmap_x);
@@ -119,13 +208,15 @@ __global__ void __launch_bounds__(w8::THREADS)
     for (int i = 0; i < min(stages, nkb); ++i) rla_tma_prefetch_l2_2d(&tmap_w, (kb0 + i) * w8::BK, n0);
   }
   if (warp == 1) {
-    rla_tmem_alloc(&tmem_base, COLS);
+    rla_tmem_alloc(&tmem_base, tmem_cols);
     rla_tmem_relinquish();
   }
   rla_tc_fence_before();
   __syncthreads();
   rla_tc_fence_after();
   const uint32_t tmem = tmem_base;
+  // (only now, so that a dependent launch cannot take the TMEM columns first)
+  rla_griddep_launch_dependents();
   rla_griddep_wait();  // before any read of what an earlier kernel may have written
 
   bool ok = true;
@@ -137,8 +228,8 @@ __global__ void __launch_bounds__(w8::THREADS)
         if (i >= stages &&
             !rla_mbar_wait(&empty[s], ((i / stages) - 1) & 1, RLA_DEVERR_TIMEOUT_SLOT_EMPTY, abort_flag))
           break;
-        uint8_t* slot = ring + (uint32_t)s * STAGE;
-        rla_mbar_arrive_expect_tx(&full[s], STAGE);
+        uint8_t* slot = ring + (uint32_t)s * stage;
+        rla_mbar_arrive_expect_tx(&full[s], stage);
         rla_tma_load_2d(slot, &tmap_w, &full[s], (kb0 + i) * w8::BK, n0);
         rla_tma_load_2d(slot + w8::BR * w8::BK, &tmap_x, &full[s], (kb0 + i) * w8::BK, m0);
         issued = i + 1;
@@ -150,13 +241,13 @@ __global__ void __launch_bounds__(w8::THREADS)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = rla_idesc_i8_s32(w8::BR, BT);
+      const uint32_t idesc = rla_idesc_i8_s32(w8::BR, bt);
       for (int i = 0; i < nkb && ok; ++i) {
         const int s = i % stages;
         ok = rla_mbar_wait(&full[s], (i / stages) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, abort_flag);
         if (!ok) break;
         rla_tc_fence_after();
-        const uint32_t wbase = rla_smem_u32(ring) + (uint32_t)s * STAGE;
+        const uint32_t wbase = rla_smem_u32(ring) + (uint32_t)s * stage;
         const uint32_t xbase = wbase + w8::BR * w8::BK;
 #pragma unroll
         for (int ks = 0; ks < w8::BK / 32; ++ks)
@@ -173,52 +264,60 @@ __global__ void __launch_bounds__(w8::THREADS)
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int n = n0 + row;
-    for (int c = threadIdx.x - 64; c < BT; c += 128) sx_s[c] = m0 + c < out.M ? out.sx[m0 + c] : 0.f;
-    float sw = 0.f, bias = 0.f;
-    if (n < out.N) {
-      sw = out.sw_f32 ? static_cast<const float*>(out.sw)[n] : __half2float(static_cast<const __half*>(out.sw)[n]);
-      bias = out.bias_kind == 0 ? 0.f
-             : out.bias_kind == 1 ? __half2float(static_cast<const __half*>(out.bias)[n])
-                                  : static_cast<const float*>(out.bias)[n];
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps: sx_s is complete
+    const int t = threadIdx.x - 64;
+    const int cols = min(bt, out.M - m0);
+    for (int c = t; c < cols; c += 128) sx_s[c] = out.sx[m0 + c];
+    const float sw = n < out.N ? w8a8_channel(out.sw, out.sw_f32 ? 2 : 1, n) : 0.f;
+    const float bias = n < out.N ? w8a8_channel(out.bias, out.bias_kind, n) : 0.f;
+    sw_s[row] = sw;
+    bias_s[row] = bias;
+    rla_named_bar_sync(1, 128);  // the epilogue warps
     ok = rla_mbar_wait(&dfull, 0, RLA_DEVERR_TIMEOUT_ACCUM, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     rla_tc_fence_after();
-    int* part = reinterpret_cast<int*>(ring);  // [BT][128]: every copy and MMA of the ring is done
+    int* part = reinterpret_cast<int*>(ring);  // [bt][128]: every copy and MMA of the ring is done
     if (ok) {
-      const int cols = min(BT, out.M - m0);
 #pragma unroll 1
-      for (int j = 0; j < cols; j += LD) {
-        uint32_t d[LD];
-        if constexpr (LD == 16)
-          rla_tmem_ld_32x32b_x16(tmem + lane_addr + j, d);
-        else
-          rla_tmem_ld_32x32b_x32(tmem + lane_addr + j, d);
+      for (int j = 0; j < cols; j += 16) {
+        uint32_t d[16];
+        rla_tmem_ld_32x32b_x16(tmem + lane_addr + j, d);
         rla_tmem_wait_ld();
         if (splits > 1) {
 #pragma unroll
-          for (int i = 0; i < LD; ++i) part[(j + i) * w8::BR + row] = static_cast<int>(d[i]);
+          for (int i = 0; i < 16; ++i) part[(j + i) * w8::BR + row] = static_cast<int>(d[i]);
         } else if (n < out.N) {
           __half* yp = out.y + (int64_t)(m0 + j) * out.ldy + n;
 #pragma unroll
-          for (int i = 0; i < LD; ++i)
-            if (j + i < cols)
-              yp[i * out.ldy] = __float2half_rn(fmaf(static_cast<float>(static_cast<int>(d[i])) * sw, sx_s[j + i], bias));
+          for (int i = 0; i < 16; ++i)
+            if (j + i < cols) yp[i * out.ldy] = w8a8_value(static_cast<int>(d[i]), sw, sx_s[j + i], bias);
         }
       }
     }
     if (splits > 1) {
       __syncwarp();
       rla_cluster_sync();
-      if (ok && n < out.N) {
-        const int cols = min(BT, out.M - m0);
-        const uint32_t mine = rla_smem_u32(part) + row * 4;
-        for (int c = rank; c < cols; c += splits) {
-          int sum = 0;
-          for (int r = 0; r < splits; ++r)
-            sum += static_cast<int>(rla_ld_dsmem_u32(mine + c * (w8::BR * 4), r));
-          out.y[(int64_t)(m0 + c) * out.ldy + n] = __float2half_rn(fmaf(static_cast<float>(sum) * sw, sx_s[c], bias));
+      // thread t: four channels (16 bytes) of the columns rank + splits * (t / 32 + 4 i);
+      // all ranks' loads are issued before the first is used
+      if (ok) {
+        const int r4 = lane * 4;
+        const uint32_t mine = rla_smem_u32(part) + r4 * 4;
+        for (int c = rank + splits * (t >> 5); c < cols; c += splits * 4) {
+          int4 v[w8::MAX_SPLITS];
+#pragma unroll
+          for (int r = 0; r < w8::MAX_SPLITS; ++r)
+            if (r < splits) v[r] = rla_ld_cluster_int4(rla_mapa(mine + c * (w8::BR * 4), r));
+          int4 sum = v[0];
+#pragma unroll
+          for (int r = 1; r < w8::MAX_SPLITS; ++r)
+            if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+          const float sx = sx_s[c];
+          const float4 w4 = *reinterpret_cast<const float4*>(sw_s + r4), b4 = *reinterpret_cast<const float4*>(bias_s + r4);
+          __half* yp = out.y + (int64_t)(m0 + c) * out.ldy + n0 + r4;
+          const __half h[4] = {w8a8_value(sum.x, w4.x, sx, b4.x), w8a8_value(sum.y, w4.y, sx, b4.y),
+                               w8a8_value(sum.z, w4.z, sx, b4.z), w8a8_value(sum.w, w4.w, sx, b4.w)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n0 + r4 + i < out.N) yp[i] = h[i];
         }
       }
       __syncwarp();
@@ -233,7 +332,176 @@ __global__ void __launch_bounds__(w8::THREADS)
   __syncthreads();
   if (warp == 1) {
     rla_tc_fence_after();
-    rla_tmem_dealloc(tmem, COLS);
+    rla_tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// Tile number -> (channel tile, token tile): token tiles in groups that stay
+// in L2 while all channel tiles pass over them.
+struct W8Order {
+  int tiles_n, tiles_m, group;
+  RLA_DEVFN void at(int tile, int& tn, int& tm) const {
+    const int per = group * tiles_n;
+    const int g = tile / per, in = tile - g * per;
+    const int rows = min(group, tiles_m - g * group);
+    tn = in / rows;
+    tm = g * group + in - tn * rows;
+  }
+};
+
+struct W8PairShared {
+  alignas(1024) uint8_t ring[w8::PAIR_STAGES][2 * 128 * w8::BK];  // 128 channels, then 128 tokens
+  float sx[2][w8::PAIR_ROWS];
+  uint64_t full[w8::PAIR_STAGES], empty[w8::PAIR_STAGES], dfull[2], dempty[2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::THREADS, 1)
+    w8a8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                     const W8Out out, int num_kb, const W8Order order) {
+  extern __shared__ uint8_t smem_raw[];
+  W8PairShared& sm =
+      *reinterpret_cast<W8PairShared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int STAGES = w8::PAIR_STAGES;
+  constexpr uint32_t HALF = 128 * w8::BK;  // bytes of one operand's part in one CTA
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = rla_cluster_ctarank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = order.tiles_n * order.tiles_m;
+  volatile int* abort_flag = &sm.abort_flag;
+
+  if (threadIdx.x == 0) {
+    rla_tma_prefetch_desc(&tmap_w);
+    rla_tma_prefetch_desc(&tmap_x);
+    for (int s = 0; s < STAGES; ++s) {
+      rla_mbar_init(&sm.full[s], 1);   // the leader's expect_tx; both CTAs' bytes count on the leader's barrier
+      rla_mbar_init(&sm.empty[s], 1);  // the leader's commit, to both
+    }
+    for (int a = 0; a < 2; ++a) {
+      rla_mbar_init(&sm.dfull[a], 1);
+      rla_mbar_init(&sm.dempty[a], 8);  // (leader's) four epilogue warps of each CTA
+    }
+    rla_mbar_init(&sm.drain, 1);
+    sm.abort_flag = 0;
+    rla_fence_barrier_init();
+  }
+  if (warp == 1) {
+    rla_tmem2_alloc(&sm.tmem_base, 512);
+    rla_tmem2_relinquish();
+  }
+  rla_tc_fence_before();
+  __syncthreads();
+  rla_cluster_sync();  // the other CTA's barriers are ready
+  rla_tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  rla_griddep_launch_dependents();
+  rla_griddep_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;  // k blocks since the start, over all tiles
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        int tn, tm;
+        order.at(tile, tn, tm);
+        const int n0 = tn * w8::PAIR_ROWS + static_cast<int>(rank) * 128;
+        const int m0 = tm * w8::PAIR_ROWS + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (it >= STAGES) {
+            ok = rla_mbar_wait_cluster(&sm.empty[s], ((it / STAGES) - 1) & 1, RLA_DEVERR_TIMEOUT_SLOT_EMPTY, abort_flag);
+            if (!ok) break;
+          }
+          if (rank == 0) rla_mbar_arrive_expect_tx(&sm.full[s], 4 * HALF);
+          const uint32_t bar = rla_mapa(rla_smem_u32(&sm.full[s]), 0);
+          rla_tma2_load_2d(sm.ring[s], &tmap_w, bar, kb * w8::BK, n0);
+          rla_tma2_load_2d(sm.ring[s] + HALF, &tmap_x, bar, kb * w8::BK, m0);
+        }
+      }
+      if (*abort_flag && rank == 0)  // both CTAs' copies count here, and both stay until the end
+        for (int i = max(0, it - STAGES); i < it; ++i)
+          rla_mbar_wait_cluster(&sm.full[i % STAGES], (i / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = rla_idesc_i8_s32(w8::PAIR_ROWS, w8::PAIR_ROWS);
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
+        const int a = n & 1;
+        if (n >= 2) {
+          ok = rla_mbar_wait_cluster(&sm.dempty[a], ((n >> 1) - 1) & 1, RLA_DEVERR_TIMEOUT_ACCUM, abort_flag);
+          if (!ok) break;
+          rla_tc_fence_after();
+        }
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const int s = it % STAGES;
+          ok = rla_mbar_wait_cluster(&sm.full[s], (it / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, abort_flag);
+          if (!ok) break;
+          rla_tc_fence_after();
+          const uint32_t wbase = rla_smem_u32(sm.ring[s]);
+#pragma unroll
+          for (int ks = 0; ks < w8::BK / 32; ++ks)
+            rla_umma2_ss_i8(tmem + a * 256, rla_smem_desc_sw128(wbase + ks * 32),
+                            rla_smem_desc_sw128(wbase + HALF + ks * 32), idesc, (kb | ks) != 0 ? 1u : 0u);
+          rla_umma2_commit(&sm.empty[s]);
+        }
+        rla_umma2_commit(&sm.dfull[a]);
+      }
+      if (!ok) {  // no MMA writes TMEM after its release
+        rla_umma2_commit(&sm.drain);
+        rla_mbar_wait_cluster(&sm.drain, 0, RLA_DEVERR_TIMEOUT_ACCUM, nullptr);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const int t = threadIdx.x - 64;
+    int n_tile = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++n_tile) {
+      const int a = n_tile & 1;
+      int tn, tm;
+      order.at(tile, tn, tm);
+      const int n = tn * w8::PAIR_ROWS + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+      const int m0 = tm * w8::PAIR_ROWS;
+      const int cols = min(w8::PAIR_ROWS, out.M - m0);
+      for (int c = t; c < cols; c += 128) sm.sx[a][c] = out.sx[m0 + c];
+      const float sw = n < out.N ? w8a8_channel(out.sw, out.sw_f32 ? 2 : 1, n) : 0.f;
+      const float bias = n < out.N ? w8a8_channel(out.bias, out.bias_kind, n) : 0.f;
+      rla_named_bar_sync(1, 128);
+      bool ok = rla_mbar_wait_cluster(&sm.dfull[a], (n_tile >> 1) & 1, RLA_DEVERR_TIMEOUT_ACCUM, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      // (a warp that gave up still meets the others at the barrier above)
+      if (!ok) continue;
+      rla_tc_fence_after();
+#pragma unroll 1
+      for (int j = 0; j < cols; j += 16) {
+        uint32_t d[16];
+        rla_tmem_ld_32x32b_x16(tmem + lane_addr + a * 256 + j, d);
+        rla_tmem_wait_ld();
+        if (n < out.N) {
+          __half* yp = out.y + (int64_t)(m0 + j) * out.ldy + n;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (j + i < cols) yp[i * out.ldy] = w8a8_value(static_cast<int>(d[i]), sw, sm.sx[a][j + i], bias);
+        }
+      }
+      rla_tc_fence_before();
+      __syncwarp();
+      if (lane == 0) rla_mbar_arrive_cluster(rla_mapa(rla_smem_u32(&sm.dempty[a]), 0));
+    }
+  }
+  rla_tc_fence_before();
+  __syncthreads();
+  // both CTAs are through: nothing reads or writes the other's shared memory or TMEM any more
+  rla_cluster_sync();
+  if (warp == 1) {
+    rla_tc_fence_after();
+    rla_tmem2_dealloc(tmem, 512);
   }
 }
 
@@ -256,23 +524,29 @@ __global__ void w8a8_align_rows_kernel(const int8_t* __restrict__ src, int64_t l
 }
 
 struct W8Plan {
+  bool pair = false;
   int bt = 0, splits = 1, per_sm = 1, stages = 0;
   int grid_x = 0, grid_y = 0;
   size_t smem = 0;
 };
 
-// Token columns: the smallest MMA shape that holds the batch (256 above 128).
 // K slices and CTAs per SM: the pair with the shortest estimated time, in k
 // blocks of one SM's share of the memory system -- rounds of resident CTAs x
 // the k blocks a CTA streams, plus a fixed cost a round.
 static W8Plan w8a8_plan(int64_t M, int64_t N, int64_t K) {
   W8Plan p;
-  p.bt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  p.grid_x = static_cast<int>((N + w8::BR - 1) / w8::BR);
-  p.grid_y = static_cast<int>((M + p.bt - 1) / p.bt);
-  const int64_t tiles = (int64_t)p.grid_x * p.grid_y;
-  const int kb = static_cast<int>((K + w8::BK - 1) / w8::BK);
   const int sms = device_sm_count();
+  const int kb = static_cast<int>((K + w8::BK - 1) / w8::BK);
+  const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256);
+  if (M > 128 && 2 * pair_tiles >= sms) {
+    p.pair = true;
+    return p;
+  }
+  // Token tiles of equal width, a multiple of 16 columns, at most 256.
+  p.grid_y = static_cast<int>((M + 255) / 256);
+  p.bt = static_cast<int>(((M + p.grid_y - 1) / p.grid_y + 15) / 16 * 16);
+  p.grid_x = static_cast<int>((N + w8::BR - 1) / w8::BR);
+  const int64_t tiles = (int64_t)p.grid_x * p.grid_y;
   const int stage = w8::stage_bytes(p.bt);
   double best = 0;
   for (int c = 1; c <= (p.bt <= 32 ? 4 : p.bt <= 64 ? 2 : 1); ++c) {
@@ -294,22 +568,44 @@ static W8Plan w8a8_plan(int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
-template <int BT>
-static cudaError_t launch_w8a8_cfg(const W8Plan& p, const CUtensorMap& tw, const CUtensorMap& tx, const W8Out& out,
-                                   int num_kb, cudaStream_t s) {
-  auto kern = w8a8_split_kernel<BT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
-  if (e != cudaSuccess) return e;
+static cudaError_t launch_w8a8(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const W8Out& out, int64_t K,
+                               cudaStream_t s) {
+  const W8Plan p = w8a8_plan(out.M, out.N, K);
+  CUtensorMap tw, tx;
+  if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, (uint64_t)K, (uint64_t)out.N, (uint64_t)ldw, w8::BK, w8::BR,
+                    CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)K, (uint64_t)out.M, (uint64_t)ldx, w8::BK,
+                    p.pair ? 128 : p.bt, CU_TENSOR_MAP_SWIZZLE_128B))
+    return cudaErrorInvalidValue;
+  const int num_kb = static_cast<int>((K + w8::BK - 1) / w8::BK);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.grid_x, p.grid_y, p.splits);
   cfg.blockDim = dim3(w8::THREADS);
-  cfg.dynamicSmemBytes = p.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (p.pair) {
+    W8Order order;
+    order.tiles_n = (out.N + w8::PAIR_ROWS - 1) / w8::PAIR_ROWS;
+    order.tiles_m = (out.M + w8::PAIR_ROWS - 1) / w8::PAIR_ROWS;
+    // a group of token tiles takes at most 32 MB of L2
+    order.group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(order.tiles_m, (32 << 20) / (w8::PAIR_ROWS * K))));
+    const int64_t tiles = (int64_t)order.tiles_n * order.tiles_m;
+    if (tiles > INT32_MAX / 2) return cudaErrorInvalidConfiguration;
+    const int pairs = static_cast<int>(std::min<int64_t>(tiles, device_sm_count() / 2));
+    cfg.gridDim = dim3(2 * pairs);
+    cfg.dynamicSmemBytes = sizeof(W8PairShared) + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(w8a8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)cfg.dynamicSmemBytes);
+    if (e != cudaSuccess) return e;
+    return cudaLaunchKernelEx(&cfg, w8a8_pair_kernel, tw, tx, out, num_kb, order);
+  }
+  cudaError_t e = cudaFuncSetAttribute(w8a8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(p.grid_x, p.grid_y, p.splits);
+  cfg.dynamicSmemBytes = p.smem;
   if (p.splits > 1) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 1;
@@ -317,26 +613,9 @@ static cudaError_t launch_w8a8_cfg(const W8Plan& p, const CUtensorMap& tw, const
     attr[1].val.clusterDim.z = static_cast<unsigned>(p.splits);
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, kern, tw, tx, out, num_kb, p.stages);
-}
-
-static cudaError_t launch_w8a8(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const W8Out& out, int64_t K,
-                               cudaStream_t s) {
-  const W8Plan p = w8a8_plan(out.M, out.N, K);
-  CUtensorMap tw, tx;
-  if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, (uint64_t)K, (uint64_t)out.N, (uint64_t)ldw, w8::BK, w8::BR,
-                    CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)K, (uint64_t)out.M, (uint64_t)ldx, w8::BK, p.bt,
-                    CU_TENSOR_MAP_SWIZZLE_128B))
-    return cudaErrorInvalidValue;
-  const int num_kb = static_cast<int>((K + w8::BK - 1) / w8::BK);
-  switch (p.bt) {
-    case 16: return launch_w8a8_cfg<16>(p, tw, tx, out, num_kb, s);
-    case 32: return launch_w8a8_cfg<32>(p, tw, tx, out, num_kb, s);
-    case 64: return launch_w8a8_cfg<64>(p, tw, tx, out, num_kb, s);
-    case 128: return launch_w8a8_cfg<128>(p, tw, tx, out, num_kb, s);
-    default: return launch_w8a8_cfg<256>(p, tw, tx, out, num_kb, s);
-  }
+  int cols = 32;  // TMEM columns: a power of two
+  while (cols < p.bt) cols *= 2;
+  return cudaLaunchKernelEx(&cfg, w8a8_split_kernel, tw, tx, out, num_kb, p.stages, p.bt, cols);
 }
 
 static bool w8a8_rows_aligned(const void* p, int64_t ld, int64_t rows) {

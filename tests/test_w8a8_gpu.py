@@ -195,7 +195,7 @@ def _gemm_check(q, sx, w, sw, b=None):
 
 
 # tokens around every tile width, channels and K around a tile and a k block
-@pytest.mark.parametrize("M", [1, 15, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 600])
+@pytest.mark.parametrize("M", [1, 15, 16, 17, 32, 33, 64, 65, 100, 128, 129, 256, 257, 600])
 @pytest.mark.parametrize("N,K", [(1, 16), (127, 112), (129, 128), (256, 144), (1000, 2064)])
 def test_w8a8_sizes(cuda_lib, M, N, K):
     g = _gen(M * 7 + N * 3 + K)
@@ -208,6 +208,16 @@ def test_w8a8_sizes(cuda_lib, M, N, K):
 def test_w8a8_configurations(cuda_lib, M, N, K):
     from rotalabs_accel_b200 import _capi
     _gemm_check(*_gemm_case(M, N, K, _gen(M + N + K), torch.float32, torch.float16))
+    assert _capi.device_error() == 0
+
+
+# many tiles: the persistent CTA pairs, ragged on every side, one to some tiles
+# a pair, one k block, more tokens than a group of tiles holds
+@pytest.mark.parametrize("M,N,K", [(2000, 3001, 272), (300, 9500, 144), (20000, 130, 1040), (1025, 5000, 16),
+                                   (4097, 2049, 128), (700, 20000, 4112), (9000, 1500, 4096)])
+def test_w8a8_many_tiles(cuda_lib, M, N, K):
+    from rotalabs_accel_b200 import _capi
+    _gemm_check(*_gemm_case(M, N, K, _gen(M + N + K), torch.float16, torch.float32 if M % 2 else None))
     assert _capi.device_error() == 0
 
 
