@@ -6,23 +6,35 @@
 //                                  c * sd * (Wd a) ),  c = p or p / sum p
 //
 // Bound by the weights of the experts that some token chose: each byte is
-// read once, by one warp, and meets all tokens that chose its expert.  The
-// products are "swap-AB" tensor-core products like the decode GEMM's: 16
+// read once, by one warp, and meets all tokens that chose its expert.
+//
+// Stream.  Every warp has a ring of its own in shared memory, filled by bulk
+// copies that its lanes issue themselves: a stage is 256 bytes of 16 weight
+// rows.  One CTA of 16 warps an SM keeps 16 x STAGES x 4 KB on their way
+// (latency x bandwidth needs about 50 KB), through every reduction and change
+// of expert, and no warp waits for another one's data.  (Loads into registers,
+// with the warps of a CTA splitting K and meeting after every 16 rows, took
+// 119 us for one token, 2 of 8 experts of 4096 x 14336.)  The work is cut into
+// stages and every CTA, and every warp of it, gets an equal, contiguous run;
+// a block of rows that spans warps is added up in shared memory.
+//
+// Products are "swap-AB" tensor-core products like the decode GEMM's: 16
 // weight rows are the rows of an m16n8k16 MMA, tokens its columns, int8 ->
 // fp16 in registers, fp32 sums.  Column = token index, so no gather: a lane
 // whose token did not choose the expert loads nothing and multiplies zeros,
 // and 8-token tiles without any such token are skipped.
 //
 // Routing.  Which weights to read is not known before the logits are, so
-// the whole GPU waits for them.  Each cluster of 8 CTAs computes all logits by
+// the whole GPU waits for them.  Each cluster of 4 CTAs computes all logits by
 // itself (K split over its CTAs, joined through distributed shared memory):
-// no grid-wide barrier, one kernel launch less, and 1/8 of the router's bytes
+// no grid-wide barrier, one kernel launch less, and 1/4 of the router's bytes
 // an SM.  A choice between two experts is a border, so the partial logits
-// (fp32 sums over 1/8 of K or less) are added in 64 bits.  Ties go to the
+// (fp32 sums over 1/4 of K or less) are added in 64 bits.  Ties go to the
 // lower index.
 //
 // Every sum has a fixed order: results are bit-reproducible.
 #include <algorithm>
+#include <atomic>
 
 #include "rla_common.cuh"
 #include "rla_internal.h"
@@ -30,13 +42,21 @@
 namespace rla {
 
 namespace moe {
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
-constexpr int CLUSTER = 8;
+constexpr int WARPS = 16;
+constexpr int THREADS = 32 * WARPS;
+constexpr int CLUSTER = 4;
 constexpr int MAX_T = 32;
 constexpr int MAX_E = 256;
 constexpr int MAX_K = 32;  // top_k
 constexpr int MAX_SPLITS = 8;
+constexpr int KB = 256;  // bytes of a weight row in a stage: four 64-wide chunks
+// Row r of a stage: even rows first, then odd rows 64 bytes further on, so
+// that the eight lanes of a 128-bit load phase (two rows x 64 bytes) hit all
+// 32 banks.
+constexpr int ODD = 8 * KB + 64;
+constexpr int SLOT = 16 * KB + 64;
+__host__ __device__ constexpr int up_stages(int nt) { return 3; }
+__host__ __device__ constexpr int down_stages(int nt) { return nt >= 2 ? 2 : 3; }  // (its reduction takes 8 KB x NT)
 }  // namespace moe
 
 struct MoeArgs {
@@ -63,20 +83,82 @@ RLA_DEVFN float moe_scale(const void* p, int f32, int64_t i) {
 }
 // Store into CTA `rank`'s copy of the shared variable at `p`.
 RLA_DEVFN void rla_st_dsmem_u32(const void* p, uint32_t rank, uint32_t v) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(rla_mapa(rla_smem_u32(p), rank)), "r"(v) : "memory");
+}
+RLA_DEVFN double rla_ld_dsmem_f64(const void* p, uint32_t rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(rla_mapa(rla_smem_u32(p), rank)) : "memory");
+  return v;
+}
+RLA_DEVFN float rla_ld_dsmem_f32(const void* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(rla_mapa(rla_smem_u32(p), rank)) : "memory");
+  return v;
+}
+// `bytes` contiguous bytes (a multiple of 16, both ends 16-byte aligned) into this CTA's shared memory.
+RLA_DEVFN void rla_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(rla_smem_u32(bar))
+               : "memory");
+}
+RLA_DEVFN uint4 rla_lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
 }
 
 // What every CTA of both kernels knows of the routing.
 struct MoeRoute {
   int ids[moe::MAX_T * moe::MAX_K];
   float coef[moe::MAX_T * moe::MAX_K];
-  uint32_t mask[moe::MAX_E];                // tokens that chose expert e
-  uint8_t slot[moe::MAX_E][moe::MAX_T];     // at which of their top_k places
-  short active[moe::MAX_E];                 // experts that some token chose, in order
+  uint32_t mask[moe::MAX_E];             // tokens that chose expert e
+  uint8_t slot[moe::MAX_E][moe::MAX_T];  // at which of their top_k places
+  short active[moe::MAX_E];              // experts that some token chose, in order
   int warp_count[moe::WARPS];
   int num_active;
+  int abort_flag;
+};
+
+template <int STAGES>
+struct MoeShared {
+  alignas(128) uint8_t ring[moe::WARPS][STAGES][moe::SLOT];
+  uint64_t full[moe::WARPS][STAGES];
+  MoeRoute r;
+};
+
+// A warp's ring: issue() starts the copy of the next stage, wait() waits for
+// the oldest; the caller keeps at most STAGES in flight.
+template <int STAGES>
+struct MoeRing {
+  uint32_t base;
+  uint64_t* full;
+  int put = 0, got = 0;   // stages issued, stages waited for
+  RLA_DEVFN void init(MoeShared<STAGES>& sm, int warp, int lane) {
+    base = rla_smem_u32(sm.ring[warp]);
+    full = sm.full[warp];
+    if (lane < STAGES) rla_mbar_init(&full[lane], 1);
+  }
+  // row: this lane's row at the stage's first byte (lanes 0-15)
+  RLA_DEVFN void issue(const int8_t* row, uint32_t bytes, int lane) {
+    const int s = put++ % STAGES;
+    if (lane == 0) rla_mbar_arrive_expect_tx(&full[s], 16 * bytes);
+    __syncwarp();
+    if (lane < 16) rla_bulk_load(base + s * moe::SLOT + (lane >> 1) * moe::KB + (lane & 1) * moe::ODD, row, bytes, &full[s]);
+  }
+  // `at`: the stage's address for the row of lane / 4 (its row + 8 is 4 * KB on); false: gave up
+  RLA_DEVFN bool wait(int lane, volatile int* abort_flag, uint32_t& at) {
+    const int s = got % STAGES;
+    const bool ok = rla_mbar_wait(&full[s], (got / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    ++got;
+    const int gr = lane >> 2;
+    at = base + s * moe::SLOT + (gr >> 1) * moe::KB + (gr & 1) * moe::ODD + (lane & 3) * 16;
+    return true;
+  }
+  // after a wait that gave up: the copies in flight land before the CTA leaves
+  RLA_DEVFN void drain() {
+    for (; got < put; ++got) rla_mbar_wait(&full[got % STAGES], (got / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
+  }
 };
 
 // ids / coef -> mask, slot, active.  All threads of the CTA.
@@ -106,41 +188,73 @@ RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
   __syncthreads();
 }
 
-// One 64-wide k chunk: 16 weight rows (rows g and g + 8 in wa) times NT tiles
-// of 8 tokens.  The k order inside the fragments follows the 16-byte loads
-// (rla_skinny.cu); `tiles` has a bit for each 8-token tile with a token.
-template <int NT>
-RLA_DEVFN void moe_chunk_mma(float (&acc)[NT][4], const uint4 (&wa)[2], const uint4 (&xb)[NT][2], uint32_t tiles) {
-  const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&wa[0]);
-  const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&wa[1]);
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    uint32_t a0, a1, a2, a3;
-    rla_i8x4_to_h2x2(w0[s], a0, a2);
-    rla_i8x4_to_h2x2(w1[s], a1, a3);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (NT > 1 && !(tiles >> t & 1)) continue;
-      const uint32_t* xw = reinterpret_cast<const uint32_t*>(&xb[t][0]);
-      rla_mma_16816(acc[t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
-    }
-  }
-}
-
 RLA_DEVFN uint32_t moe_tiles(uint32_t mask) {
   return (mask & 0xffu ? 1u : 0u) | (mask & 0xff00u ? 2u : 0u) | (mask & 0xff0000u ? 4u : 0u) |
          (mask & 0xff000000u ? 8u : 0u);
 }
 
-// Partial logits of this CTA's K slice: part[t][e], fp32.  Warps take 16
-// experts each; a lane's fragment columns are its 8-token tile's tokens.
+// One stage: 16 weight rows x up to 256 k (four 64-wide chunks) in shared
+// memory at `w` (this lane's 16 bytes of row lane / 4, chunk 0) times NT tiles
+// of 8 tokens.  xp[t]: this lane's activations of token 8 t + lane / 4 at the
+// stage's first k + 16 * (lane % 4).  The k order inside the fragments follows
+// the 16-byte pieces (rla_skinny.cu).  `bytes`: k of the stage; what lies
+// behind them is stale int8 data, finite, times zeros.  `mask`, `tiles`: the
+// expert's tokens and the 8-token tiles that have one.
 template <int NT>
-RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part) {
+RLA_DEVFN void moe_stage(float (&acc)[NT][4], uint32_t w, const __half* const (&xp)[NT], int bytes, uint32_t mask,
+                         uint32_t tiles, int lane) {
+  const int gr = lane >> 2, q = lane & 3;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  constexpr int AHEAD = NT == 1 ? 4 : 2;  // chunks of activations held in registers
+  uint4 xb[AHEAD][NT][2];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool has = (mask >> (t * 8 + gr) & 1) && c * 64 + q * 16 < bytes;
+      xb[c % AHEAD][t][0] = has ? rla_ldg_keep(xp[t] + c * 64) : zero;
+      xb[c % AHEAD][t][1] = has ? rla_ldg_keep(xp[t] + c * 64 + 8) : zero;
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < AHEAD; ++c) load(c);
+#pragma unroll
+  for (int c = 0; c < moe::KB / 64; ++c) {
+    if (c * 64 >= bytes) break;
+    const uint4 wa = rla_lds128(w + c * 64), wb = rla_lds128(w + c * 64 + 4 * moe::KB);
+    const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&wa);
+    const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&wb);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      uint32_t a0, a1, a2, a3;
+      rla_i8x4_to_h2x2(w0[s], a0, a2);
+      rla_i8x4_to_h2x2(w1[s], a1, a3);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (NT > 1 && !(tiles >> t & 1)) continue;
+        const uint32_t* xw = reinterpret_cast<const uint32_t*>(&xb[c % AHEAD][t][0]);
+        rla_mma_16816(acc[t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
+      }
+    }
+    if (c + AHEAD < moe::KB / 64) load(c + AHEAD);
+  }
+}
+
+// Logits of this CTA's K slice, v[t][e] in 64 bits.  A warp takes 16 experts
+// and, where there are fewer 16-expert tiles than warps, a part of the slice;
+// `part` [parts][T][E] (fp32) is scratch.  A lane's fragment columns are its
+// 8-token tile's tokens.
+template <int NT>
+RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part, double* v) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, q = lane & 3;
+  const int etiles = (g.E + 15) / 16;  // at most WARPS
+  const int parts = moe::WARPS / etiles;
   const int blocks = (g.H + 31) / 32;  // 32 halves = one 8-half load of each of 4 lanes
-  const int b0 = blocks * rank / moe::CLUSTER, b1 = blocks * (rank + 1) / moe::CLUSTER;
-  for (int e0 = warp * 16; e0 < g.E; e0 += moe::WARPS * 16) {
+  if (warp < etiles * parts) {
+    const int e0 = warp % etiles * 16, sub = warp / etiles;
+    const int slices = moe::CLUSTER * parts, slice = rank * parts + sub;
+    const int b0 = static_cast<int>((int64_t)blocks * slice / slices);
+    const int b1 = static_cast<int>((int64_t)blocks * (slice + 1) / slices);
     const int r0 = min(e0 + gr, g.E - 1), r1 = min(e0 + gr + 8, g.E - 1);
     const __half* w0 = g.router + (int64_t)r0 * g.H + q * 8;
     const __half* w1 = g.router + (int64_t)r1 * g.H + q * 8;
@@ -164,100 +278,136 @@ RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = e0 + gr + 8 * (i >> 1), tok = t * 8 + 2 * q + (i & 1);
-        if (e < g.E && tok < g.T) part[tok * g.E + e] = acc[t][i];
+        if (e < g.E && tok < g.T) part[(sub * g.T + tok) * g.E + e] = acc[t][i];
       }
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < g.T * g.E; p += moe::THREADS) {
+    double sum = 0;
+    for (int j = 0; j < parts; ++j) sum += static_cast<double>(part[j * g.T * g.E + p]);
+    v[p] = sum;
   }
 }
 
-// Top-k and softmax of the tokens t = rank, rank + 8, ... (one a warp), from
-// all ranks' partial logits; ids and coef go into every CTA of the cluster.
-RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, const float* part, MoeRoute& r) {
+// Softmax and choice of the tokens t = rank, rank + CLUSTER, ..., from all
+// ranks' partial logits; ids and coef go into every CTA of the cluster.  An
+// expert's place is the number of experts before it (larger logit, or equal
+// and a lower index); a NaN counts as the smallest, so that every place is
+// taken.
+struct MoeChoose {
+  double v[moe::MAX_T / moe::CLUSTER][moe::MAX_E];
+  double top[moe::MAX_T / moe::CLUSTER];
+  float total[moe::MAX_T / moe::CLUSTER];
+  short chosen[moe::MAX_T / moe::CLUSTER][moe::MAX_K];
+};
+RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, const double* mine, MoeChoose& c, MoeRoute& r) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int PER = moe::MAX_E / 32;
-  for (int t = rank + moe::CLUSTER * warp; t < g.T; t += moe::CLUSTER * moe::WARPS) {
-    double v[PER];
+  const int tokens = g.T > rank ? (g.T - rank + moe::CLUSTER - 1) / moe::CLUSTER : 0;
+  for (int p = threadIdx.x; p < tokens * g.E; p += moe::THREADS) {
+    const int tl = p / g.E, e = p - tl * g.E;
+    double sum = 0;
+#pragma unroll
+    for (int d = 0; d < moe::CLUSTER; ++d) sum += rla_ld_dsmem_f64(mine + (rank + tl * moe::CLUSTER) * g.E + e, d);
+    c.v[tl][e] = sum;
+  }
+  __syncthreads();
+  static_assert(moe::WARPS >= moe::MAX_T / moe::CLUSTER, "a warp a token");
+  if (warp < tokens) {
     double top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = lane + 32 * i;
-      v[i] = -INFINITY;
-      if (e < g.E) {
-        double sum = 0;
-        const uint32_t at = rla_smem_u32(part + t * g.E + e);
-#pragma unroll
-        for (int c = 0; c < moe::CLUSTER; ++c) {
-          uint32_t remote;
-          float f;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(c));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(remote) : "memory");
-          sum += static_cast<double>(f);
-        }
-        v[i] = sum;
-        top = fmax(top, sum);  // (drops NaN)
-      }
-    }
+    for (int e = lane; e < g.E; e += 32) top = fmax(top, c.v[warp][e]);  // (drops NaN)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // softmax relative to the largest; a NaN logit makes the sum NaN
-    float total = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i < g.E) total += expf(static_cast<float>(v[i] - top));
+    float total = 0.f;  // a NaN logit makes it NaN
+    for (int e = lane; e < g.E; e += 32) total += expf(static_cast<float>(c.v[warp][e] - top));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    // k rounds of "largest not yet taken, the lower index on a tie"; NaN
-    // counts as the smallest, so that every round finds an expert
-    uint32_t taken = 0;
-    float chosen = 0.f;  // sum of the chosen, in the order of choice
-    int my_id = 0;
-    float my_p = 0.f;
-    for (int j = 0; j < g.top_k; ++j) {
-      double bv = -INFINITY;
-      int bi = INT32_MAX;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        const double c = isnan(v[i]) ? -INFINITY : v[i];
-        if (e < g.E && !(taken >> i & 1) && (bi == INT32_MAX || c > bv)) bv = c, bi = e;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double ov = __shfl_xor_sync(0xffffffffu, bv, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-        if (oi != INT32_MAX && (bi == INT32_MAX || ov > bv || (ov == bv && oi < bi))) bv = ov, bi = oi;
-      }
-      const float p = expf(static_cast<float>(bv - top)) / total;
-      if (lane == (bi & 31)) taken |= 1u << (bi >> 5);
-      chosen += p;
-      if (lane == j) my_id = bi, my_p = p;
+    if (lane == 0) c.top[warp] = top, c.total[warp] = total;
+  }
+  for (int p = threadIdx.x; p < tokens * g.E; p += moe::THREADS) {
+    const int tl = p / g.E, e = p - tl * g.E;
+    const double me = isnan(c.v[tl][e]) ? -INFINITY : c.v[tl][e];
+    int place = 0;
+#pragma unroll 8
+    for (int o = 0; o < g.E; ++o) {
+      const double other = c.v[tl][o];
+      place += other > me || (o < e && !(other < me) && (other == me || me == -INFINITY)) ? 1 : 0;
     }
-    if (lane < g.top_k) {
-      const float c = g.renorm ? my_p / chosen : my_p;
-      for (int d = 0; d < moe::CLUSTER; ++d) {
-        rla_st_dsmem_u32(&r.ids[t * g.top_k + lane], d, static_cast<uint32_t>(my_id));
-        rla_st_dsmem_u32(&r.coef[t * g.top_k + lane], d, __float_as_uint(c));
-      }
+    if (place < g.top_k) c.chosen[tl][place] = static_cast<short>(e);
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < tokens * g.top_k; p += moe::THREADS) {
+    const int tl = p / g.top_k, j = p - tl * g.top_k;
+    const double top = c.top[tl];
+    const float total = c.total[tl];
+    float sum = 0.f, mine_p = 0.f;
+    for (int o = 0; o < g.top_k; ++o) {
+      const float pr = expf(static_cast<float>(c.v[tl][c.chosen[tl][o]] - top)) / total;
+      sum += pr;
+      if (o == j) mine_p = pr;
+    }
+    const float coef = g.renorm ? mine_p / sum : mine_p;
+    const int at = (rank + tl * moe::CLUSTER) * g.top_k + j;
+#pragma unroll
+    for (int d = 0; d < moe::CLUSTER; ++d) {
+      rla_st_dsmem_u32(&r.ids[at], d, static_cast<uint32_t>(c.chosen[tl][j]));
+      rla_st_dsmem_u32(&r.coef[at], d, __float_as_uint(coef));
     }
   }
+}
+
+// A unit of the gate/up kernel: 8 gate rows and the same 8 up rows of one expert.
+template <int NT>
+RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int i0, const float (&acc)[NT][4], int lane) {
+  const int gr = lane >> 2, q = lane & 3;
+  const uint32_t mask = r.mask[e];
+  const int i = i0 + gr;
+  const float sg = moe_scale(g.s_gate, g.scale_f32, (int64_t)e * g.I + i);
+  const float su = moe_scale(g.s_up, g.scale_f32, (int64_t)e * g.I + i);
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tok = t * 8 + 2 * q + j;
+      if (mask >> tok & 1) {
+        const float gate = acc[t][j] * sg, up = acc[t][2 + j] * su;
+        // the down product's tensor-core operand is fp16: one rounding
+        g.a[((int64_t)tok * g.top_k + r.slot[e][tok]) * g.I + i] =
+            __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
+      }
+    }
 }
 
 template <int NT>
-__global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THREADS, 2)
+__global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THREADS, 1)
     moe_gate_up_kernel(const MoeArgs g) {
-  extern __shared__ __align__(16) uint8_t moe_smem[];
-  MoeRoute& r = *reinterpret_cast<MoeRoute*>(moe_smem);
-  float* part = reinterpret_cast<float*>(moe_smem + sizeof(MoeRoute));  // [T][E]
-  __shared__ float red[moe::WARPS - 1][NT * 4][32];
+  constexpr int STAGES = moe::up_stages(NT);
+  using Shared = MoeShared<STAGES>;
+  extern __shared__ uint8_t moe_smem[];
+  Shared& sm = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  MoeRoute& r = sm.r;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, q = lane & 3;
   const int rank = static_cast<int>(rla_cluster_ctarank());
 
+  MoeRing<STAGES> ring;
+  ring.init(sm, warp, lane);
+  if (threadIdx.x == 0) r.abort_flag = 0;
+  rla_fence_barrier_init();
   rla_griddep_launch_dependents();
   rla_griddep_wait();
-  moe_logits<NT>(g, rank, part);
+
+  // routing; its scratch lies in the ring, which is not in use yet
+  constexpr int PART = moe::WARPS * 16 * 8 * NT * 4;  // [parts][T][E] floats at most
+  constexpr int LOGITS = 8 * NT * moe::MAX_E * 8;
+  static_assert(PART + LOGITS + sizeof(MoeChoose) <= sizeof(sm.ring), "routing scratch fits the ring");
+  float* part = reinterpret_cast<float*>(&sm.ring[0][0][0]);
+  double* logits = reinterpret_cast<double*>(&sm.ring[0][0][0] + PART);
+  MoeChoose& choose = *reinterpret_cast<MoeChoose*>(&sm.ring[0][0][0] + PART + LOGITS);
+  moe_logits<NT>(g, rank, part, logits);
   rla_cluster_sync();
-  moe_choose(g, rank, part, r);
+  moe_choose(g, rank, logits, choose, r);
   rla_cluster_sync();
+  rla_fence_proxy_async();  // plain accesses to the ring come before the copies into it
   if (blockIdx.x == 0)
     for (int p = threadIdx.x; p < g.T * g.top_k; p += moe::THREADS) {
       g.ids[p] = r.ids[p];
@@ -265,86 +415,105 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
     }
   moe_build_lists(r, g.T, g.E, g.top_k);
 
-  // Units of 8 gate rows and the same 8 up rows; the warps split K.
-  const int groups = (g.I + 7) / 8;
-  const int units = r.num_active * groups;
-  const int chunks = (g.H + 63) / 64;
-  constexpr int U = NT >= 4 ? 2 : 4;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int e = r.active[u / groups];
-    const int i0 = (u % groups) * 8;
+  // This CTA's units, and of their stages this warp's run.
+  const int groups = g.I / 8;
+  const int per = (g.H + moe::KB - 1) / moe::KB;  // stages of a unit
+  const int64_t units = (int64_t)r.num_active * groups;
+  const int u0 = static_cast<int>(units * blockIdx.x / gridDim.x);
+  const int u1 = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x);
+  const int64_t items = (int64_t)(u1 - u0) * per;
+  const int64_t i0 = items * warp / moe::WARPS, i1 = items * (warp + 1) / moe::WARPS;
+  const int n = static_cast<int>(i1 - i0);
+
+  int pu = u0 + static_cast<int>(i0 / per), ps = static_cast<int>(i0 % per);  // the copies' place
+  auto put = [&]() {
+    const int e = r.active[pu / groups];
+    const int8_t* w = (lane & 8) ? g.w_up : g.w_gate;
+    const int8_t* row = w + ((int64_t)e * g.I + pu % groups * 8 + (lane & 7)) * g.H + ps * moe::KB;
+    ring.issue(row, min(moe::KB, g.H - ps * moe::KB), lane);
+    if (++ps == per) ps = 0, ++pu;
+  };
+  for (int i = 0; i < STAGES && i < n; ++i) put();
+
+  int cu = u0 + static_cast<int>(i0 / per), cs = static_cast<int>(i0 % per);  // the products' place
+  bool head = n > 0 && cs != 0;  // the current unit began in an earlier warp
+  bool ok = true, tail = false, has_head = false;
+  float acc[NT][4] = {}, first[NT][4];
+  for (int i = 0; i < n; ++i) {
+    const int e = r.active[cu / groups];
     const uint32_t mask = r.mask[e];
-    const uint32_t tiles = moe_tiles(mask);
-    const int64_t row = (int64_t)e * g.I + min(i0 + gr, g.I - 1);
-    const int8_t* wg = g.w_gate + row * g.H + q * 16;
-    const int8_t* wu = g.w_up + row * g.H + q * 16;
-    float acc[NT][4] = {};
-    for (int c = warp; c < chunks; c += moe::WARPS * U) {
-      uint4 wa[U][2], xb[U][NT][2];
+    uint32_t at;
+    ok = ring.wait(lane, &r.abort_flag, at);
+    if (!ok) break;
+    const __half* xp[NT];
 #pragma unroll
-      for (int v = 0; v < U; ++v) {
-        const int k = (c + v * moe::WARPS) * 64;
-        const bool in = k + q * 16 < g.H;
-        wa[v][0] = in ? rla_ldg_stream(wg + k) : zero;
-        wa[v][1] = in ? rla_ldg_stream(wu + k) : zero;
+    for (int t = 0; t < NT; ++t) xp[t] = g.x + (int64_t)(t * 8 + gr) * g.ldx + cs * moe::KB + q * 16;
+    moe_stage<NT>(acc, at, xp, g.H - cs * moe::KB, mask, moe_tiles(mask), lane);
+    __syncwarp();
+    if (i + STAGES < n) put();
+    if (++cs == per || i + 1 == n) {
+      if (head) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int tok = t * 8 + gr;
-          const bool has = in && (mask >> tok & 1);
-          const __half* xp = g.x + (int64_t)tok * g.ldx + q * 16 + k;
-          xb[v][t][0] = has ? rla_ldg_keep(xp) : zero;
-          xb[v][t][1] = has ? rla_ldg_keep(xp + 8) : zero;
-        }
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) first[t][j] = acc[t][j];
+        has_head = true;
+        head = false;
+      } else if (cs == per) {
+        moe_finish_unit<NT>(g, r, e, cu % groups * 8, acc, lane);
+      } else {
+        tail = true;  // goes on in the next warps; acc stays
+        break;
       }
+      if (cs == per) cs = 0, ++cu;
 #pragma unroll
-      for (int v = 0; v < U; ++v) moe_chunk_mma<NT>(acc, wa[v], xb[v], tiles);
+      for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
     }
-    __syncthreads();  // the previous unit's sums have been read
-    if (warp > 0) {
+  }
+  if (!ok) ring.drain();
+  float* heads = reinterpret_cast<float*>(&sm.ring[0][0][0]);  // per warp, in its own ring, which is idle now
+  constexpr int STEP = STAGES * moe::SLOT / 4;
+  if (has_head) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) heads[warp * STEP + (t * 4 + j) * 32 + lane] = first[t][j];
+  }
+  __syncthreads();
+  if (tail && ok) {
+    const int64_t end = (int64_t)(cu - u0 + 1) * per;  // the unit's last stage + 1
+    for (int w = warp + 1; w < moe::WARPS; ++w) {
+      const int64_t w0 = items * w / moe::WARPS, w1 = items * (w + 1) / moe::WARPS;
+      if (w0 >= end) break;
+      if (w0 == w1) continue;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[warp - 1][t * 4 + i][lane] = acc[t][i];
+        for (int j = 0; j < 4; ++j) acc[t][j] += heads[w * STEP + (t * 4 + j) * 32 + lane];
     }
-    __syncthreads();
-    if (warp == 0) {
-      const int i = i0 + gr;
-      const float sg = i < g.I ? moe_scale(g.s_gate, g.scale_f32, (int64_t)e * g.I + i) : 0.f;
-      const float su = i < g.I ? moe_scale(g.s_up, g.scale_f32, (int64_t)e * g.I + i) : 0.f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (!(tiles >> t & 1)) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int w = 0; w < moe::WARPS - 1; ++w) acc[t][j] += red[w][t * 4 + j][lane];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = t * 8 + 2 * q + j;
-          if ((mask >> tok & 1) && i < g.I) {
-            const float gate = acc[t][j] * sg, up = acc[t][2 + j] * su;
-            // the down product's tensor-core operand is fp16: one rounding
-            g.a[((int64_t)tok * g.top_k + r.slot[e][tok]) * g.I + i] =
-                __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
-          }
-        }
-      }
-    }
+    moe_finish_unit<NT>(g, r, r.active[cu / groups], cu % groups * 8, acc, lane);
   }
 }
 
-// One CTA: 16 output rows, and of the (active expert, 64-wide chunk of I)
-// list the `splits`-th part, of which each warp takes a contiguous run.
+// Blocks of 16 output rows; of a block's (active expert, stage) list each
+// warp of each of the `splits` CTAs of the cluster takes an equal run.
 template <int NT>
-__global__ void __launch_bounds__(moe::THREADS, 2) moe_down_kernel(const MoeArgs g) {
-  extern __shared__ __align__(16) uint8_t moe_smem[];
-  MoeRoute& r = *reinterpret_cast<MoeRoute*>(moe_smem);
-  __shared__ __align__(16) float red[moe::WARPS][NT * 4][32];
+__global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs g) {
+  constexpr int STAGES = moe::down_stages(NT);
+  struct Shared : MoeShared<STAGES> {
+    float red[moe::WARPS][NT * 4][32];
+  };
+  extern __shared__ uint8_t moe_smem[];
+  Shared& sm = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  MoeRoute& r = sm.r;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, q = lane & 3;
   const int splits = gridDim.y, split = blockIdx.y;  // == cluster rank
 
+  MoeRing<STAGES> ring;
+  ring.init(sm, warp, lane);
+  if (threadIdx.x == 0) r.abort_flag = 0;
+  rla_fence_barrier_init();
   rla_griddep_launch_dependents();
   rla_griddep_wait();
   for (int p = threadIdx.x; p < g.T * g.top_k; p += moe::THREADS) {
@@ -354,107 +523,129 @@ __global__ void __launch_bounds__(moe::THREADS, 2) moe_down_kernel(const MoeArgs
   __syncthreads();
   moe_build_lists(r, g.T, g.E, g.top_k);
 
-  const int n0 = blockIdx.x * 16;
-  const int na = min(n0 + gr, g.H - 1), nb = min(n0 + gr + 8, g.H - 1);
-  const int chunks = (g.I + 63) / 64;
-  const int64_t items = (int64_t)r.num_active * chunks;
+  const int blocks = g.H / 16;
+  const int per = (g.I + moe::KB - 1) / moe::KB;
+  const int64_t items = (int64_t)r.num_active * per;
   const int parts = splits * moe::WARPS, mine = split * moe::WARPS + warp;
-  int64_t c0 = items * mine / parts;
-  const int64_t c1 = items * (mine + 1) / parts;
-  constexpr int U = NT >= 4 ? 2 : 4;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  float sum[NT][4] = {};
-  while (c0 < c1) {
-    const int ai = static_cast<int>(c0 / chunks);
-    const int e = r.active[ai];
-    const int kc0 = static_cast<int>(c0 - (int64_t)ai * chunks);
-    const int kc1 = static_cast<int>(min((int64_t)chunks, c1 - (int64_t)ai * chunks));
-    const uint32_t mask = r.mask[e];
-    const uint32_t tiles = moe_tiles(mask);
-    const int8_t* w0 = g.w_down + ((int64_t)e * g.H + na) * g.I + q * 16;
-    const int8_t* w1 = g.w_down + ((int64_t)e * g.H + nb) * g.I + q * 16;
-    const __half* ap[NT];
+  const int i0 = static_cast<int>(items * mine / parts), n = static_cast<int>(items * (mine + 1) / parts) - i0;
+  const int a0 = i0 / per, s0 = i0 % per;
+
+  // the copies run through all blocks of this CTA without a break
+  int pb = blockIdx.x, pa = a0, ps = s0, pi = 0;
+  auto put = [&]() {
+    if (n == 0 || pb >= blocks) return;
+    const int8_t* row =
+        g.w_down + ((int64_t)r.active[pa] * g.H + pb * 16 + (lane & 7) + ((lane & 8) ? 8 : 0)) * g.I + ps * moe::KB;
+    ring.issue(row, min(moe::KB, g.I - ps * moe::KB), lane);
+    if (++ps == per) ps = 0, ++pa;
+    if (++pi == n) pi = 0, pa = a0, ps = s0, pb += gridDim.x;
+  };
+  for (int i = 0; i < STAGES; ++i) put();
+
+  bool ok = true;
+  for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const int na = b * 16 + gr, nb = na + 8;
+    float sum[NT][4] = {}, acc[NT][4] = {};
+    int ca = a0, cs = s0;
+    for (int i = 0; i < n && ok; ++i) {
+      const int e = r.active[ca];
+      const uint32_t mask = r.mask[e];
+      const __half* xp[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int tok = t * 8 + gr;
-      const int64_t arow = (mask >> tok & 1) ? (int64_t)tok * g.top_k + r.slot[e][tok] : 0;
-      ap[t] = g.a + arow * g.I + q * 16;
-    }
-    float acc[NT][4] = {};
-    for (int c = kc0; c < kc1; c += U) {
-      uint4 wa[U][2], xb[U][NT][2];
-#pragma unroll
-      for (int v = 0; v < U; ++v) {
-        const int k = (c + v) * 64;
-        const bool in = c + v < kc1 && k + q * 16 < g.I;
-        wa[v][0] = in ? rla_ldg_stream(w0 + k) : zero;
-        wa[v][1] = in ? rla_ldg_stream(w1 + k) : zero;
+      for (int t = 0; t < NT; ++t) {
+        const int tok = t * 8 + gr;
+        const int64_t arow = (mask >> tok & 1) ? (int64_t)tok * g.top_k + r.slot[e][tok] : 0;
+        xp[t] = g.a + arow * g.I + cs * moe::KB + q * 16;
+      }
+      uint32_t at;
+      ok = ring.wait(lane, &r.abort_flag, at);
+      if (!ok) break;
+      moe_stage<NT>(acc, at, xp, g.I - cs * moe::KB, mask, moe_tiles(mask), lane);
+      __syncwarp();
+      put();
+      if (++cs == per || i + 1 == n) {
+        // this expert's part: x channel scale x token coefficient
+        const float sa = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + na);
+        const float sb = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + nb);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const bool has = in && (mask >> (t * 8 + gr) & 1);
-          xb[v][t][0] = has ? rla_ldg_keep(ap[t] + k) : zero;
-          xb[v][t][1] = has ? rla_ldg_keep(ap[t] + k + 8) : zero;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int tok = t * 8 + 2 * q + j;
+            if (mask >> tok & 1) {
+              const float c = r.coef[tok * g.top_k + r.slot[e][tok]];
+              sum[t][j] = fmaf(acc[t][j] * sa, c, sum[t][j]);
+              sum[t][2 + j] = fmaf(acc[t][2 + j] * sb, c, sum[t][2 + j]);
+            }
+          }
+          acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
         }
-      }
-#pragma unroll
-      for (int v = 0; v < U; ++v) moe_chunk_mma<NT>(acc, wa[v], xb[v], tiles);
-    }
-    // this expert's part: x channel scale x token coefficient
-    const float s0 = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + na);
-    const float s1 = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + nb);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int tok = t * 8 + 2 * q + j;
-        if (mask >> tok & 1) {
-          const float c = r.coef[tok * g.top_k + r.slot[e][tok]];
-          sum[t][j] = fmaf(acc[t][j] * s0, c, sum[t][j]);
-          sum[t][2 + j] = fmaf(acc[t][2 + j] * s1, c, sum[t][2 + j]);
-        }
+        cs = 0, ++ca;
       }
     }
-    c0 = (int64_t)ai * chunks + kc1;
-  }
-
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[warp][t * 4 + i][lane] = sum[t][i];
-  __syncthreads();
-  // the CTA's sum into red[0] (each thread its own entries), then the ranks'
-  for (int p = threadIdx.x; p < NT * 4 * 32; p += moe::THREADS) {
-    float v = red[0][p / 32][p % 32];
-#pragma unroll
-    for (int w = 1; w < moe::WARPS; ++w) v += red[w][p / 32][p % 32];
-    red[0][p / 32][p % 32] = v;
-  }
-  if (splits > 1)
-    rla_cluster_sync();
-  else
+      for (int i = 0; i < 4; ++i) sm.red[warp][t * 4 + i][lane] = sum[t][i];
     __syncthreads();
-  if (split == 0) {
+    // the CTA's sum into red[0] (each thread its own entries), then the ranks'
     for (int p = threadIdx.x; p < NT * 4 * 32; p += moe::THREADS) {
-      const int l = p % 32, ti = p / 32, t = ti / 4, i = ti % 4;
-      float v = red[0][ti][l];
-      const uint32_t at = rla_smem_u32(&red[0][ti][l]);
-      for (int c = 1; c < splits; ++c) {
-        uint32_t remote;
-        float f;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(c));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(remote) : "memory");
-        v += f;
-      }
-      const int n = n0 + (l >> 2) + 8 * (i >> 1), tok = t * 8 + 2 * (l & 3) + (i & 1);
-      if (n < g.H && tok < g.T) g.y[(int64_t)tok * g.ldy + n] = __float2half_rn(v);
+      float v = sm.red[0][p / 32][p % 32];
+#pragma unroll
+      for (int w = 1; w < moe::WARPS; ++w) v += sm.red[w][p / 32][p % 32];
+      sm.red[0][p / 32][p % 32] = v;
     }
+    if (splits > 1) rla_cluster_sync();
+    if (split == 0) {
+      for (int p = threadIdx.x; p < NT * 4 * 32; p += moe::THREADS) {
+        const int l = p % 32, ti = p / 32, t = ti / 4, i = ti % 4;
+        float v = sm.red[0][ti][l];
+        for (int c = 1; c < splits; ++c) v += rla_ld_dsmem_f32(&sm.red[0][ti][l], c);
+        const int row = b * 16 + (l >> 2) + 8 * (i >> 1), tok = t * 8 + 2 * (l & 3) + (i & 1);
+        if (tok < g.T) g.y[(int64_t)tok * g.ldy + row] = __float2half_rn(v);
+      }
+    }
+    if (splits > 1)
+      rla_cluster_sync();  // no CTA goes on while rank 0 may still read it
+    else
+      __syncthreads();
   }
-  if (splits > 1) rla_cluster_sync();  // no CTA leaves while rank 0 may still read it
+  if (!ok) ring.drain();
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+// Clusters of the gate/up kernel that run at once: its grid.  Per device.
+template <int NT>
+static int moe_up_clusters(size_t smem) {
+  static std::atomic<int> cache[64];
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
+  if (dev >= 0) {
+    const int c = cache[dev].load(std::memory_order_relaxed);
+    if (c > 0) return c;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(moe::CLUSTER);
+  cfg.blockDim = dim3(moe::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = moe::CLUSTER;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, moe_gate_up_kernel<NT>, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    return std::max(1, device_sm_count() / moe::CLUSTER);
+  }
+  if (dev >= 0) cache[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 template <int NT>
 static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   const int sms = device_sm_count();
@@ -467,21 +658,23 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
 
-  cfg.dynamicSmemBytes = sizeof(MoeRoute) + (size_t)g.T * g.E * 4;
+  cfg.dynamicSmemBytes = sizeof(MoeShared<moe::up_stages(NT)>) + 128;
   cudaError_t e = cudaFuncSetAttribute(moe_gate_up_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)cfg.dynamicSmemBytes);
   if (e != cudaSuccess) return e;
-  const int64_t most = (int64_t)std::min(g.E, g.T * g.top_k) * ((g.I + 7) / 8);
-  int64_t ctas = std::min<int64_t>(2 * sms, most);
-  ctas = (ctas + moe::CLUSTER - 1) / moe::CLUSTER * moe::CLUSTER;
-  cfg.gridDim = dim3((unsigned)ctas);
+  const int64_t most = (int64_t)std::min(g.E, g.T * g.top_k) * (g.I / 8);  // units, at most
+  const int64_t clusters = std::min<int64_t>(moe_up_clusters<NT>(cfg.dynamicSmemBytes),
+                                             (most + moe::CLUSTER - 1) / moe::CLUSTER);
+  cfg.gridDim = dim3((unsigned)(clusters * moe::CLUSTER));
   e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, g);
   if (e != cudaSuccess) return e;
 
-  cfg.dynamicSmemBytes = sizeof(MoeRoute);
-  const int rows = (g.H + 15) / 16;
-  int splits = std::max(1, std::min(moe::MAX_SPLITS, 2 * sms / rows));
-  cfg.gridDim = dim3(rows, splits);
+  cfg.dynamicSmemBytes = sizeof(MoeShared<moe::down_stages(NT)>) + sizeof(float) * moe::WARPS * NT * 4 * 32 + 256;
+  e = cudaFuncSetAttribute(moe_down_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+  if (e != cudaSuccess) return e;
+  const int blocks = g.H / 16;
+  const int splits = std::max(1, std::min(moe::MAX_SPLITS, sms / blocks));
+  cfg.gridDim = dim3(splits > 1 ? blocks : std::min(blocks, sms), splits);
   if (splits > 1) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 1;
