@@ -19,10 +19,11 @@
 // a block of rows that spans warps is added up in shared memory.
 //
 // Products are "swap-AB" tensor-core products like the decode GEMM's: 16
-// weight rows are the rows of an m16n8k16 MMA, tokens its columns, int8 ->
-// fp16 in registers, fp32 sums.  Column = token index, so no gather: a lane
-// whose token did not choose the expert loads nothing and multiplies zeros,
-// and 8-token tiles without any such token are skipped.
+// weight rows are the rows of an m16n8k16 MMA, the tokens that chose the
+// expert its columns (1, 2 or 4 tiles of 8), int8 -> fp16 in registers, fp32
+// sums.  A column with no token repeats another one's activations and is
+// dropped: columns of a product do not mix, and loads without conditions
+// keep the instructions of a 1 KB piece near the 40 of its conversion.
 //
 // Routing.  Which weights to read is not known before the logits are, so
 // the whole GPU waits for them.  Each cluster of 4 CTAs computes all logits by
@@ -55,8 +56,8 @@ constexpr int KB = 256;  // bytes of a weight row in a stage: four 64-wide chunk
 // 32 banks.
 constexpr int ODD = 8 * KB + 64;
 constexpr int SLOT = 16 * KB + 64;
-__host__ __device__ constexpr int up_stages(int nt) { return 3; }
-__host__ __device__ constexpr int down_stages(int nt) { return nt >= 2 ? 2 : 3; }  // (its reduction takes 8 KB x NT)
+constexpr int MAX_STAGES = 3;
+constexpr size_t SMEM = 227 * 1024;  // of a CTA
 }  // namespace moe
 
 struct MoeArgs {
@@ -107,119 +108,141 @@ RLA_DEVFN uint4 rla_lds128(uint32_t addr) {
   return v;
 }
 
-// What every CTA of both kernels knows of the routing.
+// What every CTA of both kernels knows of the routing.  A pair p = token *
+// top_k + place stands for (token, expert ids[p]); entry[] lists the pairs by
+// expert, the tokens of an expert in order, and token[] their tokens.
 struct MoeRoute {
   int ids[moe::MAX_T * moe::MAX_K];
   float coef[moe::MAX_T * moe::MAX_K];
-  uint32_t mask[moe::MAX_E];             // tokens that chose expert e
-  uint8_t slot[moe::MAX_E][moe::MAX_T];  // at which of their top_k places
-  short active[moe::MAX_E];              // experts that some token chose, in order
-  int warp_count[moe::WARPS];
+  uint32_t mask[moe::MAX_E];  // tokens that chose expert e
+  short begin[moe::MAX_E];    // first entry of expert e
+  short active[moe::MAX_E];   // experts that some token chose, in order
+  short entry[moe::MAX_T * moe::MAX_K];
+  uint8_t token[moe::MAX_T * moe::MAX_K];
+  int warp_count[moe::WARPS], warp_entries[moe::WARPS];
   int num_active;
   int abort_flag;
 };
 
-template <int STAGES>
+// Shared memory of both kernels: routing, barriers, a buffer for partial sums
+// (16 warps x 16 values for each column of the 8-token tiles), the warps' rings.
 struct MoeShared {
-  alignas(128) uint8_t ring[moe::WARPS][STAGES][moe::SLOT];
-  uint64_t full[moe::WARPS][STAGES];
   MoeRoute r;
+  uint64_t full[moe::WARPS][moe::MAX_STAGES];
 };
+__host__ __device__ constexpr size_t moe_sums_offset() { return (sizeof(MoeShared) + 127) & ~size_t(127); }
+__host__ __device__ constexpr int moe_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
+__host__ __device__ constexpr size_t moe_ring_offset(int T) { return moe_sums_offset() + (size_t)moe_tiles(T) * 8192; }
+__host__ __device__ constexpr size_t moe_smem_bytes(int T, int stages) {
+  return 128 + moe_ring_offset(T) + (size_t)moe::WARPS * stages * moe::SLOT;
+}
 
 // A warp's ring: issue() starts the copy of the next stage, wait() waits for
-// the oldest; the caller keeps at most STAGES in flight.
-template <int STAGES>
+// the oldest; the caller keeps at most `stages` in flight.
 struct MoeRing {
   uint32_t base;
   uint64_t* full;
-  int put = 0, got = 0;   // stages issued, stages waited for
-  RLA_DEVFN void init(MoeShared<STAGES>& sm, int warp, int lane) {
-    base = rla_smem_u32(sm.ring[warp]);
+  int stages, flying = 0;          // copies issued and not waited for
+  int put_slot = 0, get_slot = 0, phase = 0;
+  RLA_DEVFN MoeRing(uint8_t* ring, MoeShared& sm, int warp, int lane, int n) : stages(n) {
+    base = rla_smem_u32(ring + (size_t)warp * n * moe::SLOT);
     full = sm.full[warp];
-    if (lane < STAGES) rla_mbar_init(&full[lane], 1);
+    if (lane < n) rla_mbar_init(&full[lane], 1);
   }
   // row: this lane's row at the stage's first byte (lanes 0-15)
   RLA_DEVFN void issue(const int8_t* row, uint32_t bytes, int lane) {
-    const int s = put++ % STAGES;
-    if (lane == 0) rla_mbar_arrive_expect_tx(&full[s], 16 * bytes);
+    if (lane == 0) rla_mbar_arrive_expect_tx(&full[put_slot], 16 * bytes);
     __syncwarp();
-    if (lane < 16) rla_bulk_load(base + s * moe::SLOT + (lane >> 1) * moe::KB + (lane & 1) * moe::ODD, row, bytes, &full[s]);
+    if (lane < 16)
+      rla_bulk_load(base + put_slot * moe::SLOT + (lane >> 1) * moe::KB + (lane & 1) * moe::ODD, row, bytes, &full[put_slot]);
+    put_slot = put_slot + 1 == stages ? 0 : put_slot + 1;
+    ++flying;
+  }
+  RLA_DEVFN bool landed(volatile int* abort_flag) {
+    const bool ok = rla_mbar_wait(&full[get_slot], phase, RLA_DEVERR_TIMEOUT_TMA_FULL, abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    if (++get_slot == stages) get_slot = 0, phase ^= 1;
+    --flying;
+    return true;
   }
   // `at`: the stage's address for the row of lane / 4 (its row + 8 is 4 * KB on); false: gave up
   RLA_DEVFN bool wait(int lane, volatile int* abort_flag, uint32_t& at) {
-    const int s = got % STAGES;
-    const bool ok = rla_mbar_wait(&full[s], (got / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, abort_flag);
-    if (!__all_sync(0xffffffffu, ok)) return false;
-    ++got;
     const int gr = lane >> 2;
-    at = base + s * moe::SLOT + (gr >> 1) * moe::KB + (gr & 1) * moe::ODD + (lane & 3) * 16;
-    return true;
+    at = base + get_slot * moe::SLOT + (gr >> 1) * moe::KB + (gr & 1) * moe::ODD + (lane & 3) * 16;
+    return landed(abort_flag);
   }
   // after a wait that gave up: the copies in flight land before the CTA leaves
   RLA_DEVFN void drain() {
-    for (; got < put; ++got) rla_mbar_wait(&full[got % STAGES], (got / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
+    while (flying > 0 && landed(nullptr)) {
+    }
   }
 };
 
-// ids / coef -> mask, slot, active.  All threads of the CTA.
+// ids -> mask, begin, active, entry, token.  All threads of the CTA.
 RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   static_assert(moe::THREADS >= moe::MAX_E, "one thread an expert");
   if (tid < E) r.mask[tid] = 0;
   __syncthreads();
-  for (int p = tid; p < T * top_k; p += moe::THREADS) {
-    const int t = p / top_k;
-    atomicOr(&r.mask[r.ids[p]], 1u << t);
-    r.slot[r.ids[p]][t] = static_cast<uint8_t>(p - t * top_k);
+  for (int p = tid; p < T * top_k; p += moe::THREADS) atomicOr(&r.mask[r.ids[p]], 1u << (p / top_k));
+  __syncthreads();
+  const int count = tid < E ? __popc(r.mask[tid]) : 0;
+  const uint32_t votes = __ballot_sync(0xffffffffu, count != 0);
+  int upto = count;  // entries of this warp's experts up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
+  if (lane == 31) r.warp_count[warp] = __popc(votes), r.warp_entries[warp] = upto;
   __syncthreads();
-  const bool on = tid < E && r.mask[tid] != 0;
-  const uint32_t votes = __ballot_sync(0xffffffffu, on);
-  if ((tid & 31) == 0) r.warp_count[tid >> 5] = __popc(votes);
-  __syncthreads();
-  int before = 0, all = 0;
+  int before = 0, entries = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < moe::WARPS; ++w) {
-    before += w < (tid >> 5) ? r.warp_count[w] : 0;
+    before += w < warp ? r.warp_count[w] : 0;
+    entries += w < warp ? r.warp_entries[w] : 0;
     all += r.warp_count[w];
   }
-  if (on) r.active[before + __popc(votes & ((1u << (tid & 31)) - 1))] = static_cast<short>(tid);
+  if (count) r.active[before + __popc(votes & ((1u << lane) - 1))] = static_cast<short>(tid);
+  if (tid < E) r.begin[tid] = static_cast<short>(entries + upto - count);
   if (tid == 0) r.num_active = all;
   __syncthreads();
-}
-
-RLA_DEVFN uint32_t moe_tiles(uint32_t mask) {
-  return (mask & 0xffu ? 1u : 0u) | (mask & 0xff00u ? 2u : 0u) | (mask & 0xff0000u ? 4u : 0u) |
-         (mask & 0xff000000u ? 8u : 0u);
+  for (int p = tid; p < T * top_k; p += moe::THREADS) {
+    const int t = p / top_k, e = r.ids[p];
+    const int at = r.begin[e] + __popc(r.mask[e] & ((1u << t) - 1));
+    r.entry[at] = static_cast<short>(p);
+    r.token[at] = static_cast<uint8_t>(t);
+  }
+  __syncthreads();
 }
 
 // One stage: 16 weight rows x up to 256 k (four 64-wide chunks) in shared
 // memory at `w` (this lane's 16 bytes of row lane / 4, chunk 0) times NT tiles
-// of 8 tokens.  xp[t]: this lane's activations of token 8 t + lane / 4 at the
-// stage's first k + 16 * (lane % 4).  The k order inside the fragments follows
-// the 16-byte pieces (rla_skinny.cu).  `bytes`: k of the stage; what lies
-// behind them is stale int8 data, finite, times zeros.  `mask`, `tiles`: the
-// expert's tokens and the 8-token tiles that have one.
-template <int NT>
-RLA_DEVFN void moe_stage(float (&acc)[NT][4], uint32_t w, const __half* const (&xp)[NT], int bytes, uint32_t mask,
-                         uint32_t tiles, int lane) {
-  const int gr = lane >> 2, q = lane & 3;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  constexpr int AHEAD = NT == 1 ? 4 : 2;  // chunks of activations held in registers
+// of 8 columns.  xp[t]: this lane's activations of column 8 t + lane / 4 at
+// the stage's first k + 16 * (lane % 4).  The k order inside the fragments
+// follows the 16-byte pieces (rla_skinny.cu).  FULL: all 256 k are there;
+// otherwise `bytes` are, and behind them zeros meet stale, finite weights.
+template <int NT, bool FULL>
+RLA_DEVFN void moe_stage(float (&acc)[4][4], uint32_t w, const __half* const (&xp)[NT], int bytes, int lane) {
+  const int q = lane & 3;
+  constexpr int CHUNKS = moe::KB / 64;
+  constexpr int AHEAD = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks of activations held in registers
   uint4 xb[AHEAD][NT][2];
   auto load = [&](int c) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const bool has = (mask >> (t * 8 + gr) & 1) && c * 64 + q * 16 < bytes;
-      xb[c % AHEAD][t][0] = has ? rla_ldg_keep(xp[t] + c * 64) : zero;
-      xb[c % AHEAD][t][1] = has ? rla_ldg_keep(xp[t] + c * 64 + 8) : zero;
+      if (FULL || c * 64 + q * 16 < bytes) {
+        xb[c % AHEAD][t][0] = rla_ldg_keep(xp[t] + c * 64);
+        xb[c % AHEAD][t][1] = rla_ldg_keep(xp[t] + c * 64 + 8);
+      } else {
+        xb[c % AHEAD][t][0] = xb[c % AHEAD][t][1] = make_uint4(0, 0, 0, 0);
+      }
     }
   };
 #pragma unroll
   for (int c = 0; c < AHEAD; ++c) load(c);
 #pragma unroll
-  for (int c = 0; c < moe::KB / 64; ++c) {
-    if (c * 64 >= bytes) break;
+  for (int c = 0; c < CHUNKS; ++c) {
     const uint4 wa = rla_lds128(w + c * 64), wb = rla_lds128(w + c * 64 + 4 * moe::KB);
     const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&wa);
     const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&wb);
@@ -230,13 +253,51 @@ RLA_DEVFN void moe_stage(float (&acc)[NT][4], uint32_t w, const __half* const (&
       rla_i8x4_to_h2x2(w1[s], a1, a3);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        if (NT > 1 && !(tiles >> t & 1)) continue;
         const uint32_t* xw = reinterpret_cast<const uint32_t*>(&xb[c % AHEAD][t][0]);
         rla_mma_16816(acc[t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
       }
     }
-    if (c + AHEAD < moe::KB / 64) load(c + AHEAD);
+    if (c + AHEAD < CHUNKS) load(c + AHEAD);
   }
+}
+
+// `n` stages of one expert from the ring, from k = k0 of `width` on.  Columns
+// are the expert's tokens; the columns behind them repeat its first token and
+// are not used.  row(i): the activations' row of the expert's i-th entry.
+template <int NT, class Row, class Put>
+RLA_DEVFN bool moe_run_tiles(float (&acc)[4][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
+                             volatile int* abort_flag, const Row& row, const Put& put) {
+  const __half* xp[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int col = t * 8 + (lane >> 2);
+    xp[t] = row(col < count ? col : 0) + k0 + (lane & 3) * 16;
+  }
+  for (int i = 0; i < n; ++i) {
+    uint32_t at;
+    if (!ring.wait(lane, abort_flag, at)) return false;
+    const int bytes = width - k0 - i * moe::KB;
+    if (bytes >= moe::KB)
+      moe_stage<NT, true>(acc, at, xp, bytes, lane);
+    else
+      moe_stage<NT, false>(acc, at, xp, bytes, lane);
+    __syncwarp();
+    put();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) xp[t] += moe::KB;
+  }
+  return true;
+}
+template <class Row, class Put>
+RLA_DEVFN bool moe_run(float (&acc)[4][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
+                       volatile int* abort_flag, const Row& row, const Put& put) {
+  if (count <= 8) return moe_run_tiles<1>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+  if (count <= 16) return moe_run_tiles<2>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+  return moe_run_tiles<4>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+}
+RLA_DEVFN void moe_zero(float (&acc)[4][4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 }
 
 // Logits of this CTA's K slice, v[t][e] in 64 bits.  A warp takes 16 experts
@@ -356,41 +417,39 @@ RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, const double* mine, MoeCho
 }
 
 // A unit of the gate/up kernel: 8 gate rows and the same 8 up rows of one expert.
-template <int NT>
-RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int i0, const float (&acc)[NT][4], int lane) {
+RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int group, const float (&acc)[4][4], int lane) {
   const int gr = lane >> 2, q = lane & 3;
-  const uint32_t mask = r.mask[e];
-  const int i = i0 + gr;
+  const int i = group * 8 + gr, first = r.begin[e], count = __popc(r.mask[e]);
   const float sg = moe_scale(g.s_gate, g.scale_f32, (int64_t)e * g.I + i);
   const float su = moe_scale(g.s_up, g.scale_f32, (int64_t)e * g.I + i);
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < 4; ++t) {
+    if (t * 8 >= count) break;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int tok = t * 8 + 2 * q + j;
-      if (mask >> tok & 1) {
+      const int col = t * 8 + 2 * q + j;
+      if (col < count) {
         const float gate = acc[t][j] * sg, up = acc[t][2 + j] * su;
         // the down product's tensor-core operand is fp16: one rounding
-        g.a[((int64_t)tok * g.top_k + r.slot[e][tok]) * g.I + i] =
-            __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
+        g.a[(int64_t)r.entry[first + col] * g.I + i] = __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
       }
     }
+  }
 }
 
-template <int NT>
+template <int NT>  // tiles of 8 tokens
 __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THREADS, 1)
-    moe_gate_up_kernel(const MoeArgs g) {
-  constexpr int STAGES = moe::up_stages(NT);
-  using Shared = MoeShared<STAGES>;
+    moe_gate_up_kernel(const MoeArgs g, int stages) {
   extern __shared__ uint8_t moe_smem[];
-  Shared& sm = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  MoeShared& sm = *reinterpret_cast<MoeShared*>(smem);
   MoeRoute& r = sm.r;
+  float* heads = reinterpret_cast<float*>(smem + moe_sums_offset());
+  uint8_t* rings = smem + moe_ring_offset(g.T);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int gr = lane >> 2, q = lane & 3;
   const int rank = static_cast<int>(rla_cluster_ctarank());
 
-  MoeRing<STAGES> ring;
-  ring.init(sm, warp, lane);
+  MoeRing ring(rings, sm, warp, lane, stages);
   if (threadIdx.x == 0) r.abort_flag = 0;
   rla_fence_barrier_init();
   rla_griddep_launch_dependents();
@@ -399,10 +458,10 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   // routing; its scratch lies in the ring, which is not in use yet
   constexpr int PART = moe::WARPS * 16 * 8 * NT * 4;  // [parts][T][E] floats at most
   constexpr int LOGITS = 8 * NT * moe::MAX_E * 8;
-  static_assert(PART + LOGITS + sizeof(MoeChoose) <= sizeof(sm.ring), "routing scratch fits the ring");
-  float* part = reinterpret_cast<float*>(&sm.ring[0][0][0]);
-  double* logits = reinterpret_cast<double*>(&sm.ring[0][0][0] + PART);
-  MoeChoose& choose = *reinterpret_cast<MoeChoose*>(&sm.ring[0][0][0] + PART + LOGITS);
+  static_assert(PART + LOGITS + sizeof(MoeChoose) <= moe::WARPS * 2 * moe::SLOT, "routing scratch fits the ring");
+  float* part = reinterpret_cast<float*>(rings);
+  double* logits = reinterpret_cast<double*>(rings + PART);
+  MoeChoose& choose = *reinterpret_cast<MoeChoose*>(rings + PART + LOGITS);
   moe_logits<NT>(g, rank, part, logits);
   rla_cluster_sync();
   moe_choose(g, rank, logits, choose, r);
@@ -420,98 +479,95 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   const int per = (g.H + moe::KB - 1) / moe::KB;  // stages of a unit
   const int64_t units = (int64_t)r.num_active * groups;
   const int u0 = static_cast<int>(units * blockIdx.x / gridDim.x);
-  const int u1 = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x);
-  const int64_t items = (int64_t)(u1 - u0) * per;
-  const int64_t i0 = items * warp / moe::WARPS, i1 = items * (warp + 1) / moe::WARPS;
-  const int n = static_cast<int>(i1 - i0);
+  const int64_t items = (units * (blockIdx.x + 1) / gridDim.x - u0) * per;
+  const int64_t i0 = items * warp / moe::WARPS;
+  int left = static_cast<int>(items * (warp + 1) / moe::WARPS - i0);
+  const int unit = u0 + static_cast<int>(i0 / per);
+  int ca = unit / groups, cg = unit % groups, cs = static_cast<int>(i0 % per);  // the products' place
 
-  int pu = u0 + static_cast<int>(i0 / per), ps = static_cast<int>(i0 % per);  // the copies' place
-  auto put = [&]() {
-    const int e = r.active[pu / groups];
-    const int8_t* w = (lane & 8) ? g.w_up : g.w_gate;
-    const int8_t* row = w + ((int64_t)e * g.I + pu % groups * 8 + (lane & 7)) * g.H + ps * moe::KB;
-    ring.issue(row, min(moe::KB, g.H - ps * moe::KB), lane);
-    if (++ps == per) ps = 0, ++pu;
+  int pa = ca, pg = cg, ps = cs, to_put = left;  // the copies' place
+  const int8_t* prow = nullptr;
+  auto unit_row = [&]() {
+    return ((lane & 8) ? g.w_up : g.w_gate) + ((int64_t)r.active[pa] * g.I + pg * 8 + (lane & 7)) * g.H;
   };
-  for (int i = 0; i < STAGES && i < n; ++i) put();
-
-  int cu = u0 + static_cast<int>(i0 / per), cs = static_cast<int>(i0 % per);  // the products' place
-  bool head = n > 0 && cs != 0;  // the current unit began in an earlier warp
-  bool ok = true, tail = false, has_head = false;
-  float acc[NT][4] = {}, first[NT][4];
-  for (int i = 0; i < n; ++i) {
-    const int e = r.active[cu / groups];
-    const uint32_t mask = r.mask[e];
-    uint32_t at;
-    ok = ring.wait(lane, &r.abort_flag, at);
-    if (!ok) break;
-    const __half* xp[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) xp[t] = g.x + (int64_t)(t * 8 + gr) * g.ldx + cs * moe::KB + q * 16;
-    moe_stage<NT>(acc, at, xp, g.H - cs * moe::KB, mask, moe_tiles(mask), lane);
-    __syncwarp();
-    if (i + STAGES < n) put();
-    if (++cs == per || i + 1 == n) {
-      if (head) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) first[t][j] = acc[t][j];
-        has_head = true;
-        head = false;
-      } else if (cs == per) {
-        moe_finish_unit<NT>(g, r, e, cu % groups * 8, acc, lane);
-      } else {
-        tail = true;  // goes on in the next warps; acc stays
-        break;
-      }
-      if (cs == per) cs = 0, ++cu;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+  if (to_put > 0) prow = unit_row() + ps * moe::KB;
+  auto put = [&]() {
+    if (to_put == 0) return;
+    --to_put;
+    ring.issue(prow, min(moe::KB, g.H - ps * moe::KB), lane);
+    prow += moe::KB;
+    if (++ps == per) {
+      ps = 0;
+      if (++pg == groups) pg = 0, ++pa;
+      if (to_put > 0) prow = unit_row();
     }
+  };
+  for (int i = 0; i < stages; ++i) put();
+
+  bool head = left > 0 && cs != 0;  // the current unit began in an earlier warp
+  bool tail = false, ok = true;
+  float acc[4][4];
+  moe_zero(acc);
+  while (left > 0) {
+    const int e = r.active[ca], first = r.begin[e];
+    const int n = min(per - cs, left);
+    ok = moe_run(acc, ring, n, cs * moe::KB, g.H, __popc(r.mask[e]), lane, &r.abort_flag,
+                 [&](int i) { return g.x + r.token[first + i] * g.ldx; }, put);
+    if (!ok) break;
+    left -= n;
+    cs += n;
+    if (head) {
+      float* h = heads + warp * NT * 128 + lane;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[(t * 4 + j) * 32] = acc[t][j];
+      head = false;
+    } else if (cs == per) {
+      moe_finish_unit(g, r, e, cg, acc, lane);
+    } else {
+      tail = true;  // goes on in the next warps; acc stays
+      break;
+    }
+    if (cs == per) {
+      cs = 0;
+      if (++cg == groups) cg = 0, ++ca;
+    }
+    moe_zero(acc);
   }
   if (!ok) ring.drain();
-  float* heads = reinterpret_cast<float*>(&sm.ring[0][0][0]);  // per warp, in its own ring, which is idle now
-  constexpr int STEP = STAGES * moe::SLOT / 4;
-  if (has_head) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) heads[warp * STEP + (t * 4 + j) * 32 + lane] = first[t][j];
-  }
   __syncthreads();
   if (tail && ok) {
-    const int64_t end = (int64_t)(cu - u0 + 1) * per;  // the unit's last stage + 1
+    const int64_t end = ((int64_t)ca * groups + cg - u0 + 1) * per;  // the unit's last stage + 1
     for (int w = warp + 1; w < moe::WARPS; ++w) {
       const int64_t w0 = items * w / moe::WARPS, w1 = items * (w + 1) / moe::WARPS;
       if (w0 >= end) break;
       if (w0 == w1) continue;
+      const float* h = heads + w * NT * 128 + lane;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t][j] += heads[w * STEP + (t * 4 + j) * 32 + lane];
+        for (int j = 0; j < 4; ++j) acc[t][j] += h[(t * 4 + j) * 32];
     }
-    moe_finish_unit<NT>(g, r, r.active[cu / groups], cu % groups * 8, acc, lane);
+    moe_finish_unit(g, r, r.active[ca], cg, acc, lane);
   }
 }
 
 // Blocks of 16 output rows; of a block's (active expert, stage) list each
-// warp of each of the `splits` CTAs of the cluster takes an equal run.
-template <int NT>
-__global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs g) {
-  constexpr int STAGES = moe::down_stages(NT);
-  struct Shared : MoeShared<STAGES> {
-    float red[moe::WARPS][NT * 4][32];
-  };
+// warp of each of the `splits` CTAs of the cluster takes an equal run, and
+// adds each expert's part (x channel scale x token coefficient) to its sums
+// [T][16] in shared memory.
+__global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs g, int stages) {
   extern __shared__ uint8_t moe_smem[];
-  Shared& sm = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  MoeShared& sm = *reinterpret_cast<MoeShared*>(smem);
   MoeRoute& r = sm.r;
+  float* sums = reinterpret_cast<float*>(smem + moe_sums_offset());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, q = lane & 3;
   const int splits = gridDim.y, split = blockIdx.y;  // == cluster rank
 
-  MoeRing<STAGES> ring;
-  ring.init(sm, warp, lane);
+  MoeRing ring(smem + moe_ring_offset(g.T), sm, warp, lane, stages);
   if (threadIdx.x == 0) r.abort_flag = 0;
   rla_fence_barrier_init();
   rla_griddep_launch_dependents();
@@ -532,77 +588,71 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs
 
   // the copies run through all blocks of this CTA without a break
   int pb = blockIdx.x, pa = a0, ps = s0, pi = 0;
+  const int8_t* prow = nullptr;
+  auto block_row = [&]() { return g.w_down + ((int64_t)r.active[pa] * g.H + pb * 16 + (lane & 15)) * g.I; };
+  if (n > 0 && pb < blocks) prow = block_row() + ps * moe::KB;
   auto put = [&]() {
     if (n == 0 || pb >= blocks) return;
-    const int8_t* row =
-        g.w_down + ((int64_t)r.active[pa] * g.H + pb * 16 + (lane & 7) + ((lane & 8) ? 8 : 0)) * g.I + ps * moe::KB;
-    ring.issue(row, min(moe::KB, g.I - ps * moe::KB), lane);
-    if (++ps == per) ps = 0, ++pa;
-    if (++pi == n) pi = 0, pa = a0, ps = s0, pb += gridDim.x;
+    ring.issue(prow, min(moe::KB, g.I - ps * moe::KB), lane);
+    prow += moe::KB;
+    if (++pi == n) {
+      pi = 0, pa = a0, ps = s0, pb += gridDim.x;
+      if (pb < blocks) prow = block_row() + ps * moe::KB;
+    } else if (++ps == per) {
+      ps = 0, ++pa;
+      prow = block_row();
+    }
   };
-  for (int i = 0; i < STAGES; ++i) put();
+  for (int i = 0; i < stages; ++i) put();
 
   bool ok = true;
+  const int values = g.T * 16;
+  float* own = sums + warp * values;
   for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int na = b * 16 + gr, nb = na + 8;
-    float sum[NT][4] = {}, acc[NT][4] = {};
-    int ca = a0, cs = s0;
-    for (int i = 0; i < n && ok; ++i) {
-      const int e = r.active[ca];
-      const uint32_t mask = r.mask[e];
-      const __half* xp[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int tok = t * 8 + gr;
-        const int64_t arow = (mask >> tok & 1) ? (int64_t)tok * g.top_k + r.slot[e][tok] : 0;
-        xp[t] = g.a + arow * g.I + cs * moe::KB + q * 16;
-      }
-      uint32_t at;
-      ok = ring.wait(lane, &r.abort_flag, at);
+    for (int p = lane; p < values; p += 32) own[p] = 0.f;
+    int ca = a0, cs = s0, left = n;
+    while (left > 0 && ok) {
+      const int e = r.active[ca], first = r.begin[e], count = __popc(r.mask[e]);
+      const int m = min(per - cs, left);
+      float acc[4][4];
+      moe_zero(acc);
+      ok = moe_run(acc, ring, m, cs * moe::KB, g.I, count, lane, &r.abort_flag,
+                   [&](int i) { return g.a + (int64_t)r.entry[first + i] * g.I; }, put);
       if (!ok) break;
-      moe_stage<NT>(acc, at, xp, g.I - cs * moe::KB, mask, moe_tiles(mask), lane);
-      __syncwarp();
-      put();
-      if (++cs == per || i + 1 == n) {
-        // this expert's part: x channel scale x token coefficient
-        const float sa = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + na);
-        const float sb = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + nb);
+      const float sa = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr);
+      const float sb = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr + 8);
+      __syncwarp();  // the zeros, or another expert's sums, are in place
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+      for (int t = 0; t < 4; ++t) {
+        if (t * 8 >= count) break;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int tok = t * 8 + 2 * q + j;
-            if (mask >> tok & 1) {
-              const float c = r.coef[tok * g.top_k + r.slot[e][tok]];
-              sum[t][j] = fmaf(acc[t][j] * sa, c, sum[t][j]);
-              sum[t][2 + j] = fmaf(acc[t][2 + j] * sb, c, sum[t][2 + j]);
-            }
+        for (int j = 0; j < 2; ++j) {
+          const int col = t * 8 + 2 * q + j;
+          if (col < count) {
+            const float c = r.coef[r.entry[first + col]];
+            float* v = own + r.token[first + col] * 16 + gr;
+            v[0] = fmaf(acc[t][j] * sa, c, v[0]);
+            v[8] = fmaf(acc[t][2 + j] * sb, c, v[8]);
           }
-          acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
         }
-        cs = 0, ++ca;
       }
+      left -= m;
+      cs = 0, ++ca;
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sm.red[warp][t * 4 + i][lane] = sum[t][i];
     __syncthreads();
-    // the CTA's sum into red[0] (each thread its own entries), then the ranks'
-    for (int p = threadIdx.x; p < NT * 4 * 32; p += moe::THREADS) {
-      float v = sm.red[0][p / 32][p % 32];
+    // the CTA's sum into warp 0's (each thread its own values), then the ranks'
+    for (int p = threadIdx.x; p < values; p += moe::THREADS) {
+      float v = sums[p];
 #pragma unroll
-      for (int w = 1; w < moe::WARPS; ++w) v += sm.red[w][p / 32][p % 32];
-      sm.red[0][p / 32][p % 32] = v;
+      for (int w = 1; w < moe::WARPS; ++w) v += sums[w * values + p];
+      sums[p] = v;
     }
     if (splits > 1) rla_cluster_sync();
     if (split == 0) {
-      for (int p = threadIdx.x; p < NT * 4 * 32; p += moe::THREADS) {
-        const int l = p % 32, ti = p / 32, t = ti / 4, i = ti % 4;
-        float v = sm.red[0][ti][l];
-        for (int c = 1; c < splits; ++c) v += rla_ld_dsmem_f32(&sm.red[0][ti][l], c);
-        const int row = b * 16 + (l >> 2) + 8 * (i >> 1), tok = t * 8 + 2 * (l & 3) + (i & 1);
-        if (tok < g.T) g.y[(int64_t)tok * g.ldy + row] = __float2half_rn(v);
+      for (int p = threadIdx.x; p < values; p += moe::THREADS) {
+        float v = sums[p];
+        for (int c = 1; c < splits; ++c) v += rla_ld_dsmem_f32(&sums[p], c);
+        g.y[(int64_t)(p / 16) * g.ldy + b * 16 + p % 16] = __float2half_rn(v);
       }
     }
     if (splits > 1)
@@ -658,7 +708,9 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
 
-  cfg.dynamicSmemBytes = sizeof(MoeShared<moe::up_stages(NT)>) + 128;
+  int stages = moe::MAX_STAGES;  // 3 up to 16 tokens, 2 above
+  while (moe_smem_bytes(g.T, stages) > moe::SMEM) --stages;
+  cfg.dynamicSmemBytes = moe_smem_bytes(g.T, stages);
   cudaError_t e = cudaFuncSetAttribute(moe_gate_up_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)cfg.dynamicSmemBytes);
   if (e != cudaSuccess) return e;
@@ -666,11 +718,10 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   const int64_t clusters = std::min<int64_t>(moe_up_clusters<NT>(cfg.dynamicSmemBytes),
                                              (most + moe::CLUSTER - 1) / moe::CLUSTER);
   cfg.gridDim = dim3((unsigned)(clusters * moe::CLUSTER));
-  e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, g);
+  e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, g, stages);
   if (e != cudaSuccess) return e;
 
-  cfg.dynamicSmemBytes = sizeof(MoeShared<moe::down_stages(NT)>) + sizeof(float) * moe::WARPS * NT * 4 * 32 + 256;
-  e = cudaFuncSetAttribute(moe_down_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+  e = cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
   if (e != cudaSuccess) return e;
   const int blocks = g.H / 16;
   const int splits = std::max(1, std::min(moe::MAX_SPLITS, sms / blocks));
@@ -682,7 +733,7 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, moe_down_kernel<NT>, g);
+  return cudaLaunchKernelEx(&cfg, moe_down_kernel, g, stages);
 }
 
 static int moe_fail(int code, const char* msg) {
@@ -739,7 +790,9 @@ int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate
                   reinterpret_cast<float*>(ws + a_bytes + moe_up256(n * 4)), (int)T, (int)H, (int)I, (int)E, (int)top_k,
                   renormalize ? 1 : 0};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = T <= 8 ? launch_moe<1>(g, s) : T <= 16 ? launch_moe<2>(g, s) : launch_moe<4>(g, s);
+  const cudaError_t e = moe_tiles((int)T) == 1   ? launch_moe<1>(g, s)
+                        : moe_tiles((int)T) == 2 ? launch_moe<2>(g, s)
+                                                 : launch_moe<4>(g, s);
   if (e != cudaSuccess) {
     set_error("rla_moe: %s", cudaGetErrorString(e));
     return RLA_ERR_CUDA;

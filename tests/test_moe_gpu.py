@@ -78,7 +78,7 @@ def _check(p, k, renorm=True):
 # tokens around the 8-token tiles, widths of one 16-element piece up, E around a warp
 @pytest.mark.parametrize("T,H,I,E,k", [
     (1, 16, 16, 1, 1), (1, 64, 32, 2, 1), (2, 80, 48, 3, 3), (7, 256, 128, 8, 2), (8, 128, 272, 31, 4),
-    (9, 528, 64, 33, 2), (16, 512, 256, 64, 8), (17, 144, 96, 60, 4), (24, 96, 80, 128, 32), (31, 272, 48, 255, 3),
+    (9, 528, 64, 33, 2), (16, 512, 256, 64, 8), (17, 144, 96, 60, 4), (24, 96, 80, 128, 32), (20, 1040, 528, 2, 1), (23, 272, 1296, 3, 2), (31, 272, 48, 255, 3),
     (32, 256, 128, 256, 8), (32, 512, 512, 4, 4), (5, 4096, 1024, 4, 2), (3, 1024, 4112, 5, 1)])
 @pytest.mark.parametrize("renorm", [True, False])
 def test_sizes(cuda_lib, T, H, I, E, k, renorm):
