@@ -9,8 +9,9 @@
 // read once, by one warp, and meets all tokens that chose its expert.
 //
 // Stream.  Every warp has a ring of its own in shared memory, filled by bulk
-// copies that its lanes issue themselves: a stage is 256 bytes of 16 weight
-// rows.  One CTA of 16 warps an SM keeps 16 x STAGES x 4 KB on their way
+// tile copies that it issues itself: a stage is 256 bytes of 16 weight rows,
+// in two or four copies.  (One copy a row cost 16 issues, a third of all
+// instructions: 93 us for the case below.)  One CTA of 16 warps an SM keeps 16 x STAGES x 4 KB on their way
 // (latency x bandwidth needs about 50 KB), through every reduction and change
 // of expert, and no warp waits for another one's data.  (Loads into registers,
 // with the warps of a CTA splitting K and meeting after every 16 rows, took
@@ -39,6 +40,7 @@
 
 #include "rla_common.cuh"
 #include "rla_internal.h"
+#include "rla_tmap.cuh"
 
 namespace rla {
 
@@ -51,11 +53,10 @@ constexpr int MAX_E = 256;
 constexpr int MAX_K = 32;  // top_k
 constexpr int MAX_SPLITS = 8;
 constexpr int KB = 256;  // bytes of a weight row in a stage: four 64-wide chunks
-// Row r of a stage: even rows first, then odd rows 64 bytes further on, so
-// that the eight lanes of a 128-bit load phase (two rows x 64 bytes) hit all
-// 32 banks.
-constexpr int ODD = 8 * KB + 64;
-constexpr int SLOT = 16 * KB + 64;
+// A stage is two halves of 128 bytes x 16 rows, 128-byte swizzled by the copy
+// (16-byte piece c of row r lies at piece c ^ (r % 8)).
+constexpr int HALF = 16 * 128;
+constexpr int SLOT = 16 * KB;
 constexpr int MAX_STAGES = 3;
 constexpr size_t SMEM = 227 * 1024;  // of a CTA
 }  // namespace moe
@@ -96,12 +97,6 @@ RLA_DEVFN float rla_ld_dsmem_f32(const void* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(rla_mapa(rla_smem_u32(p), rank)) : "memory");
   return v;
 }
-// `bytes` contiguous bytes (a multiple of 16, both ends 16-byte aligned) into this CTA's shared memory.
-RLA_DEVFN void rla_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(rla_smem_u32(bar))
-               : "memory");
-}
 RLA_DEVFN uint4 rla_lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -130,11 +125,11 @@ struct MoeShared {
   MoeRoute r;
   uint64_t full[moe::WARPS][moe::MAX_STAGES];
 };
-__host__ __device__ constexpr size_t moe_sums_offset() { return (sizeof(MoeShared) + 127) & ~size_t(127); }
+__host__ __device__ constexpr size_t moe_sums_offset() { return (sizeof(MoeShared) + 1023) & ~size_t(1023); }
 __host__ __device__ constexpr int moe_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
 __host__ __device__ constexpr size_t moe_ring_offset(int T) { return moe_sums_offset() + (size_t)moe_tiles(T) * 8192; }
 __host__ __device__ constexpr size_t moe_smem_bytes(int T, int stages) {
-  return 128 + moe_ring_offset(T) + (size_t)moe::WARPS * stages * moe::SLOT;
+  return 1024 + moe_ring_offset(T) + (size_t)moe::WARPS * stages * moe::SLOT;
 }
 
 // A warp's ring: issue() starts the copy of the next stage, wait() waits for
@@ -149,14 +144,31 @@ struct MoeRing {
     full = sm.full[warp];
     if (lane < n) rla_mbar_init(&full[lane], 1);
   }
-  // row: this lane's row at the stage's first byte (lanes 0-15)
-  RLA_DEVFN void issue(const int8_t* row, uint32_t bytes, int lane) {
-    if (lane == 0) rla_mbar_arrive_expect_tx(&full[put_slot], 16 * bytes);
-    __syncwarp();
-    if (lane < 16)
-      rla_bulk_load(base + put_slot * moe::SLOT + (lane >> 1) * moe::KB + (lane & 1) * moe::ODD, row, bytes, &full[put_slot]);
+  // The next stage: columns [k, k + 256) of 16 rows, rows r0.. of map0 (all 16,
+  // or 8 of them and rows r0.. of map1).
+  template <int MAPS>
+  RLA_DEVFN void issue(const CUtensorMap* map0, const CUtensorMap* map1, int k, int r0, int width, int lane) {
+    if (lane == 0) {
+      uint64_t* bar = &full[put_slot];
+      const uint32_t to = base + put_slot * moe::SLOT;
+      const int halves = width - k > 128 ? 2 : 1;
+      rla_mbar_arrive_expect_tx(bar, halves * moe::HALF);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h == halves) break;
+        tile(to + h * moe::HALF, map0, bar, k + h * 128, r0);
+        if (MAPS == 2) tile(to + h * moe::HALF + 1024, map1, bar, k + h * 128, r0);
+      }
+    }
     put_slot = put_slot + 1 == stages ? 0 : put_slot + 1;
     ++flying;
+  }
+  RLA_DEVFN void tile(uint32_t to, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(to),
+        "l"(map), "r"(rla_smem_u32(bar)), "r"(c0), "r"(c1)
+        : "memory");
   }
   RLA_DEVFN bool landed(volatile int* abort_flag) {
     const bool ok = rla_mbar_wait(&full[get_slot], phase, RLA_DEVERR_TIMEOUT_TMA_FULL, abort_flag);
@@ -165,10 +177,9 @@ struct MoeRing {
     --flying;
     return true;
   }
-  // `at`: the stage's address for the row of lane / 4 (its row + 8 is 4 * KB on); false: gave up
-  RLA_DEVFN bool wait(int lane, volatile int* abort_flag, uint32_t& at) {
-    const int gr = lane >> 2;
-    at = base + get_slot * moe::SLOT + (gr >> 1) * moe::KB + (gr & 1) * moe::ODD + (lane & 3) * 16;
+  // `at`: the stage's address; false: gave up
+  RLA_DEVFN bool wait(volatile int* abort_flag, uint32_t& at) {
+    at = base + get_slot * moe::SLOT;
     return landed(abort_flag);
   }
   // after a wait that gave up: the copies in flight land before the CTA leaves
@@ -216,16 +227,24 @@ RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
   __syncthreads();
 }
 
+// The weight row of a stage that is row g of the MMA (and row 8 + this, of
+// its row 8 + g).  In a phase of a 128-bit load eight lanes read 64 bytes of
+// the rows of g and g + 1, g even: four rows apart, the swizzle puts them into
+// different halves of the 32 banks.
+RLA_DEVFN int moe_row(int g) { return (g >> 1) | ((g & 1) << 2); }
+
 // One stage: 16 weight rows x up to 256 k (four 64-wide chunks) in shared
-// memory at `w` (this lane's 16 bytes of row lane / 4, chunk 0) times NT tiles
-// of 8 columns.  xp[t]: this lane's activations of column 8 t + lane / 4 at
+// memory at `w` times NT tiles of 8 columns.  xp[t]: this lane's activations of column 8 t + lane / 4 at
 // the stage's first k + 16 * (lane % 4).  The k order inside the fragments
 // follows the 16-byte pieces (rla_skinny.cu).  FULL: all 256 k are there;
-// otherwise `bytes` are, and behind them zeros meet stale, finite weights.
+// otherwise `bytes` are, and behind them zeros meet zeros or stale, finite weights.
 template <int NT, bool FULL>
 RLA_DEVFN void moe_stage(float (&acc)[4][4], uint32_t w, const __half* const (&xp)[NT], int bytes, int lane) {
   const int q = lane & 3;
   constexpr int CHUNKS = moe::KB / 64;
+  const int row = moe_row(lane >> 2);
+  // 16-byte pieces q and 4 + q of the row (the 64-wide chunks of a half)
+  const uint32_t w0_at = w + row * 128 + ((q ^ row) << 4), w1_at = w + row * 128 + (((4 + q) ^ row) << 4);
   constexpr int AHEAD = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks of activations held in registers
   uint4 xb[AHEAD][NT][2];
   auto load = [&](int c) {
@@ -243,7 +262,8 @@ RLA_DEVFN void moe_stage(float (&acc)[4][4], uint32_t w, const __half* const (&x
   for (int c = 0; c < AHEAD; ++c) load(c);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const uint4 wa = rla_lds128(w + c * 64), wb = rla_lds128(w + c * 64 + 4 * moe::KB);
+    const uint32_t at = (c & 1 ? w1_at : w0_at) + (c >> 1) * moe::HALF;
+    const uint4 wa = rla_lds128(at), wb = rla_lds128(at + 1024);
     const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&wa);
     const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&wb);
 #pragma unroll
@@ -275,7 +295,7 @@ RLA_DEVFN bool moe_run_tiles(float (&acc)[4][4], MoeRing& ring, int n, int k0, i
   }
   for (int i = 0; i < n; ++i) {
     uint32_t at;
-    if (!ring.wait(lane, abort_flag, at)) return false;
+    if (!ring.wait(abort_flag, at)) return false;
     const int bytes = width - k0 - i * moe::KB;
     if (bytes >= moe::KB)
       moe_stage<NT, true>(acc, at, xp, bytes, lane);
@@ -417,11 +437,10 @@ RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, const double* mine, MoeCho
 }
 
 // A unit of the gate/up kernel: 8 gate rows and the same 8 up rows of one expert.
-RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int group, const float (&acc)[4][4], int lane) {
-  const int gr = lane >> 2, q = lane & 3;
-  const int i = group * 8 + gr, first = r.begin[e], count = __popc(r.mask[e]);
-  const float sg = moe_scale(g.s_gate, g.scale_f32, (int64_t)e * g.I + i);
-  const float su = moe_scale(g.s_up, g.scale_f32, (int64_t)e * g.I + i);
+RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int group, const float (&acc)[4][4], float sg,
+                               float su, int lane) {
+  const int q = lane & 3;
+  const int i = group * 8 + moe_row(lane >> 2), first = r.begin[e], count = __popc(r.mask[e]);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if (t * 8 >= count) break;
@@ -439,9 +458,10 @@ RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int g
 
 template <int NT>  // tiles of 8 tokens
 __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THREADS, 1)
-    moe_gate_up_kernel(const MoeArgs g, int stages) {
+    moe_gate_up_kernel(const __grid_constant__ CUtensorMap gate_map, const __grid_constant__ CUtensorMap up_map,
+                       const MoeArgs g, int stages) {
   extern __shared__ uint8_t moe_smem[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 1023) & ~uintptr_t(1023));
   MoeShared& sm = *reinterpret_cast<MoeShared*>(smem);
   MoeRoute& r = sm.r;
   float* heads = reinterpret_cast<float*>(smem + moe_sums_offset());
@@ -486,31 +506,33 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   int ca = unit / groups, cg = unit % groups, cs = static_cast<int>(i0 % per);  // the products' place
 
   int pa = ca, pg = cg, ps = cs, to_put = left;  // the copies' place
-  const int8_t* prow = nullptr;
-  auto unit_row = [&]() {
-    return ((lane & 8) ? g.w_up : g.w_gate) + ((int64_t)r.active[pa] * g.I + pg * 8 + (lane & 7)) * g.H;
-  };
-  if (to_put > 0) prow = unit_row() + ps * moe::KB;
+  int prow = to_put > 0 ? r.active[pa] * g.I + pg * 8 : 0;
   auto put = [&]() {
     if (to_put == 0) return;
     --to_put;
-    ring.issue(prow, min(moe::KB, g.H - ps * moe::KB), lane);
-    prow += moe::KB;
+    ring.issue<2>(&gate_map, &up_map, ps * moe::KB, prow, g.H, lane);
     if (++ps == per) {
       ps = 0;
-      if (++pg == groups) pg = 0, ++pa;
-      if (to_put > 0) prow = unit_row();
+      prow += 8;
+      if (++pg == groups) {
+        pg = 0, ++pa;
+        if (to_put > 0) prow = r.active[pa] * g.I;
+      }
     }
   };
   for (int i = 0; i < stages; ++i) put();
 
   bool head = left > 0 && cs != 0;  // the current unit began in an earlier warp
   bool tail = false, ok = true;
-  float acc[4][4];
+  float acc[4][4], sg = 0.f, su = 0.f;
   moe_zero(acc);
   while (left > 0) {
     const int e = r.active[ca], first = r.begin[e];
     const int n = min(per - cs, left);
+    // (read before the products, used after them)
+    const int64_t channel = (int64_t)e * g.I + cg * 8 + moe_row(lane >> 2);
+    sg = moe_scale(g.s_gate, g.scale_f32, channel);
+    su = moe_scale(g.s_up, g.scale_f32, channel);
     ok = moe_run(acc, ring, n, cs * moe::KB, g.H, __popc(r.mask[e]), lane, &r.abort_flag,
                  [&](int i) { return g.x + r.token[first + i] * g.ldx; }, put);
     if (!ok) break;
@@ -524,7 +546,7 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
         for (int j = 0; j < 4; ++j) h[(t * 4 + j) * 32] = acc[t][j];
       head = false;
     } else if (cs == per) {
-      moe_finish_unit(g, r, e, cg, acc, lane);
+      moe_finish_unit(g, r, e, cg, acc, sg, su, lane);
     } else {
       tail = true;  // goes on in the next warps; acc stays
       break;
@@ -549,7 +571,7 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[t][j] += h[(t * 4 + j) * 32];
     }
-    moe_finish_unit(g, r, r.active[ca], cg, acc, lane);
+    moe_finish_unit(g, r, r.active[ca], cg, acc, sg, su, lane);
   }
 }
 
@@ -557,14 +579,15 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
 // warp of each of the `splits` CTAs of the cluster takes an equal run, and
 // adds each expert's part (x channel scale x token coefficient) to its sums
 // [T][16] in shared memory.
-__global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs g, int stages) {
+__global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_constant__ CUtensorMap down_map,
+                                                                   const MoeArgs g, int stages) {
   extern __shared__ uint8_t moe_smem[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 127) & ~uintptr_t(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 1023) & ~uintptr_t(1023));
   MoeShared& sm = *reinterpret_cast<MoeShared*>(smem);
   MoeRoute& r = sm.r;
   float* sums = reinterpret_cast<float*>(smem + moe_sums_offset());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int gr = lane >> 2, q = lane & 3;
+  const int gr = moe_row(lane >> 2), q = lane & 3;
   const int splits = gridDim.y, split = blockIdx.y;  // == cluster rank
 
   MoeRing ring(smem + moe_ring_offset(g.T), sm, warp, lane, stages);
@@ -588,20 +611,11 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs
 
   // the copies run through all blocks of this CTA without a break
   int pb = blockIdx.x, pa = a0, ps = s0, pi = 0;
-  const int8_t* prow = nullptr;
-  auto block_row = [&]() { return g.w_down + ((int64_t)r.active[pa] * g.H + pb * 16 + (lane & 15)) * g.I; };
-  if (n > 0 && pb < blocks) prow = block_row() + ps * moe::KB;
   auto put = [&]() {
     if (n == 0 || pb >= blocks) return;
-    ring.issue(prow, min(moe::KB, g.I - ps * moe::KB), lane);
-    prow += moe::KB;
-    if (++pi == n) {
-      pi = 0, pa = a0, ps = s0, pb += gridDim.x;
-      if (pb < blocks) prow = block_row() + ps * moe::KB;
-    } else if (++ps == per) {
-      ps = 0, ++pa;
-      prow = block_row();
-    }
+    ring.issue<1>(&down_map, nullptr, ps * moe::KB, r.active[pa] * g.H + pb * 16, g.I, lane);
+    if (++ps == per) ps = 0, ++pa;
+    if (++pi == n) pi = 0, pa = a0, ps = s0, pb += gridDim.x;
   };
   for (int i = 0; i < stages; ++i) put();
 
@@ -614,13 +628,14 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const MoeArgs
     while (left > 0 && ok) {
       const int e = r.active[ca], first = r.begin[e], count = __popc(r.mask[e]);
       const int m = min(per - cs, left);
+      // (read before the products, used after them)
+      const float sa = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr);
+      const float sb = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr + 8);
       float acc[4][4];
       moe_zero(acc);
       ok = moe_run(acc, ring, m, cs * moe::KB, g.I, count, lane, &r.abort_flag,
                    [&](int i) { return g.a + (int64_t)r.entry[first + i] * g.I; }, put);
       if (!ok) break;
-      const float sa = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr);
-      const float sb = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr + 8);
       __syncwarp();  // the zeros, or another expert's sums, are in place
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -698,6 +713,12 @@ static int moe_up_clusters(size_t smem) {
 
 template <int NT>
 static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
+  CUtensorMap gate_map, up_map, down_map;
+  const uint64_t E = g.E, H = g.H, I = g.I;
+  if (!make_tmap_2d(&gate_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_gate, H, E * I, H, 128, 8, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&up_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_up, H, E * I, H, 128, 8, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&down_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_down, I, E * H, I, 128, 16, CU_TENSOR_MAP_SWIZZLE_128B))
+    return cudaErrorInvalidValue;
   const int sms = device_sm_count();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -718,7 +739,7 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   const int64_t clusters = std::min<int64_t>(moe_up_clusters<NT>(cfg.dynamicSmemBytes),
                                              (most + moe::CLUSTER - 1) / moe::CLUSTER);
   cfg.gridDim = dim3((unsigned)(clusters * moe::CLUSTER));
-  e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, g, stages);
+  e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, gate_map, up_map, g, stages);
   if (e != cudaSuccess) return e;
 
   e = cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
@@ -733,7 +754,7 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, moe_down_kernel, g, stages);
+  return cudaLaunchKernelEx(&cfg, moe_down_kernel, down_map, g, stages);
 }
 
 static int moe_fail(int code, const char* msg) {
@@ -760,8 +781,8 @@ int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate
   using namespace rla;
   static_assert(moe::MAX_T == RLA_MOE_MAX_TOKENS && moe::MAX_E == RLA_MOE_MAX_EXPERTS && moe::MAX_K == RLA_MOE_MAX_TOP_K,
                 "limits of the header");
-  if (T < 0 || H < 1 || I < 1 || E < 1 || H > (1 << 24) || I > (1 << 24))
-    return moe_fail(RLA_ERR_INVALID_ARGUMENT, "T must be >= 0, H and I in [1, 2^24], E >= 1");
+  if (T < 0 || H < 1 || I < 1 || E < 1 || H > (1 << 20) || I > (1 << 20))
+    return moe_fail(RLA_ERR_INVALID_ARGUMENT, "T must be >= 0, H and I in [1, 2^20], E >= 1");
   if (top_k < 1 || top_k > E) return moe_fail(RLA_ERR_INVALID_ARGUMENT, "top_k must be in [1, E]");
   if (T > moe::MAX_T || E > moe::MAX_E || top_k > moe::MAX_K)
     return moe_fail(RLA_ERR_UNSUPPORTED, "at most 32 tokens, 256 experts and top_k 32");
