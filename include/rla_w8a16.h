@@ -403,7 +403,7 @@ RLA_API size_t rla_w8a8_workspace_size(int64_t M, int64_t N, int64_t K);
  *           not shared by calls that may overlap
  *
  * Needs T <= RLA_MOE_MAX_TOKENS, E <= RLA_MOE_MAX_EXPERTS, top_k <=
- * RLA_MOE_MAX_TOP_K, H and I multiples of 16, 16-byte aligned x rows, router
+ * RLA_MOE_MAX_TOP_K, H and I multiples of 16 up to 2^17, 16-byte aligned x rows, router
  * and weights (else RLA_ERR_UNSUPPORTED).  Two kernels, no atomics on global
  * memory, bit-reproducible.  A token whose logits hold NaN gets NaN.
  */

@@ -35,6 +35,8 @@
 // lower index.
 //
 // Every sum has a fixed order: results are bit-reproducible.
+#include <limits.h>
+
 #include <algorithm>
 #include <atomic>
 
@@ -61,6 +63,19 @@ constexpr int MAX_STAGES = 3;
 constexpr size_t SMEM = 227 * 1024;  // of a CTA
 }  // namespace moe
 
+// What every CTA of both kernels knows of the routing.  A pair p = token *
+// top_k + place stands for (token, one of its experts); entry[] lists the
+// pairs by expert, the tokens of an expert in order, and token[] their tokens.
+struct MoeTables {
+  float coef[moe::MAX_T * moe::MAX_K];  // by pair
+  uint32_t mask[moe::MAX_E];            // tokens that chose expert e
+  short begin[moe::MAX_E];              // first entry of expert e
+  short active[moe::MAX_E];             // experts that some token chose, in order
+  short entry[moe::MAX_T * moe::MAX_K];
+  uint8_t token[moe::MAX_T * moe::MAX_K];
+  int num_active;
+};
+
 struct MoeArgs {
   const __half* x;  // [T, H], row stride ldx
   int64_t ldx;
@@ -74,9 +89,8 @@ struct MoeArgs {
   int scale_f32;
   __half* y;  // [T, H], row stride ldy
   int64_t ldy;
-  __half* a;    // workspace: [T * top_k, I]
-  int* ids;     // workspace: [T * top_k]
-  float* coef;  // workspace: [T * top_k]
+  __half* a;            // workspace: [T * top_k, I]
+  MoeTables* tables;    // workspace: the routing, for the second kernel
   int T, H, I, E, top_k, renorm;
 };
 
@@ -103,19 +117,8 @@ RLA_DEVFN uint4 rla_lds128(uint32_t addr) {
   return v;
 }
 
-// What every CTA of both kernels knows of the routing.  A pair p = token *
-// top_k + place stands for (token, expert ids[p]); entry[] lists the pairs by
-// expert, the tokens of an expert in order, and token[] their tokens.
-struct MoeRoute {
+struct MoeRoute : MoeTables {
   int ids[moe::MAX_T * moe::MAX_K];
-  float coef[moe::MAX_T * moe::MAX_K];
-  uint32_t mask[moe::MAX_E];  // tokens that chose expert e
-  short begin[moe::MAX_E];    // first entry of expert e
-  short active[moe::MAX_E];   // experts that some token chose, in order
-  short entry[moe::MAX_T * moe::MAX_K];
-  uint8_t token[moe::MAX_T * moe::MAX_K];
-  int warp_count[moe::WARPS], warp_entries[moe::WARPS];
-  int num_active;
   int abort_flag;
 };
 
@@ -189,34 +192,38 @@ struct MoeRing {
   }
 };
 
-// ids -> mask, begin, active, entry, token.  All threads of the CTA.
+// ids -> mask (zero before), begin, active, entry, token.  All threads of the CTA.
 RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  static_assert(moe::THREADS >= moe::MAX_E, "one thread an expert");
-  if (tid < E) r.mask[tid] = 0;
-  __syncthreads();
+  const int tid = threadIdx.x, lane = tid & 31;
   for (int p = tid; p < T * top_k; p += moe::THREADS) atomicOr(&r.mask[r.ids[p]], 1u << (p / top_k));
   __syncthreads();
-  const int count = tid < E ? __popc(r.mask[tid]) : 0;
-  const uint32_t votes = __ballot_sync(0xffffffffu, count != 0);
-  int upto = count;  // entries of this warp's experts up to this one
+  if (tid < 32) {  // a lane takes PER experts in a row
+    constexpr int PER = moe::MAX_E / 32;
+    int count[PER], own = 0;  // entries in the low half, experts in the high half
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) r.warp_count[warp] = __popc(votes), r.warp_entries[warp] = upto;
-  __syncthreads();
-  int before = 0, entries = 0, all = 0;
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane * PER + i;
+      count[i] = e < E ? __popc(r.mask[e]) : 0;
+      own += count[i] + (count[i] ? 1 << 16 : 0);
+    }
+    int upto = own;
 #pragma unroll
-  for (int w = 0; w < moe::WARPS; ++w) {
-    before += w < warp ? r.warp_count[w] : 0;
-    entries += w < warp ? r.warp_entries[w] : 0;
-    all += r.warp_count[w];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) r.num_active = upto >> 16;
+    int at = upto - own;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane * PER + i;
+      if (e < E) r.begin[e] = static_cast<short>(at & 0xffff);
+      if (count[i]) {
+        r.active[at >> 16] = static_cast<short>(e);
+        at += count[i] + (1 << 16);
+      }
+    }
   }
-  if (count) r.active[before + __popc(votes & ((1u << lane) - 1))] = static_cast<short>(tid);
-  if (tid < E) r.begin[tid] = static_cast<short>(entries + upto - count);
-  if (tid == 0) r.num_active = all;
   __syncthreads();
   for (int p = tid; p < T * top_k; p += moe::THREADS) {
     const int t = p / top_k, e = r.ids[p];
@@ -225,6 +232,12 @@ RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
     r.token[at] = static_cast<uint8_t>(t);
   }
   __syncthreads();
+}
+
+// Start of part i of n, parts of equal length or one more.
+RLA_DEVFN int moe_part(int total, int i, int n) {
+  const int each = total / n;
+  return each * i + min(i, total - each * n);
 }
 
 // The weight row of a stage that is row g of the MMA (and row 8 + this, of
@@ -373,60 +386,82 @@ RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part, double* v) {
 // Softmax and choice of the tokens t = rank, rank + CLUSTER, ..., from all
 // ranks' partial logits; ids and coef go into every CTA of the cluster.  An
 // expert's place is the number of experts before it (larger logit, or equal
-// and a lower index); a NaN counts as the smallest, so that every place is
-// taken.
+// and a lower index), counted by all threads at once; a NaN counts as the
+// smallest, so that every place is taken.
 struct MoeChoose {
-  double v[moe::MAX_T / moe::CLUSTER][moe::MAX_E];
+  long long key[moe::MAX_T / moe::CLUSTER][moe::MAX_E];  // the logits as integers of the same order
+  int place[moe::MAX_T / moe::CLUSTER][moe::MAX_E];
   double top[moe::MAX_T / moe::CLUSTER];
   float total[moe::MAX_T / moe::CLUSTER];
   short chosen[moe::MAX_T / moe::CLUSTER][moe::MAX_K];
+  float p[moe::MAX_T / moe::CLUSTER][moe::MAX_K];
 };
+RLA_DEVFN long long moe_key(double v) {  // (never -0: sums start from +0)
+  const long long b = __double_as_longlong(v);
+  return isnan(v) ? LLONG_MIN : b >= 0 ? b : b ^ LLONG_MAX;
+}
+RLA_DEVFN double moe_logit(long long key) {
+  return key == LLONG_MIN ? __longlong_as_double(LLONG_MAX) : __longlong_as_double(key >= 0 ? key : key ^ LLONG_MAX);
+}
 RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, const double* mine, MoeChoose& c, MoeRoute& r) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tokens = g.T > rank ? (g.T - rank + moe::CLUSTER - 1) / moe::CLUSTER : 0;
-  for (int p = threadIdx.x; p < tokens * g.E; p += moe::THREADS) {
+  const int pairs = tokens * g.E;
+  if (pairs == 0) return;  // (the whole CTA)
+  for (int p = threadIdx.x; p < pairs; p += moe::THREADS) {
     const int tl = p / g.E, e = p - tl * g.E;
-    double sum = 0;
+    double part[moe::CLUSTER], sum = 0;
 #pragma unroll
-    for (int d = 0; d < moe::CLUSTER; ++d) sum += rla_ld_dsmem_f64(mine + (rank + tl * moe::CLUSTER) * g.E + e, d);
-    c.v[tl][e] = sum;
+    for (int d = 0; d < moe::CLUSTER; ++d)
+      part[d] = rla_ld_dsmem_f64(mine + (rank + tl * moe::CLUSTER) * g.E + e, d);
+#pragma unroll
+    for (int d = 0; d < moe::CLUSTER; ++d) sum += part[d];
+    c.key[tl][e] = moe_key(sum);
+    c.place[tl][e] = 0;
   }
   __syncthreads();
   static_assert(moe::WARPS >= moe::MAX_T / moe::CLUSTER, "a warp a token");
   if (warp < tokens) {
     double top = -INFINITY;
-    for (int e = lane; e < g.E; e += 32) top = fmax(top, c.v[warp][e]);  // (drops NaN)
+    for (int e = lane; e < g.E; e += 32) top = fmax(top, moe_logit(c.key[warp][e]));  // (drops NaN)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
     float total = 0.f;  // a NaN logit makes it NaN
-    for (int e = lane; e < g.E; e += 32) total += expf(static_cast<float>(c.v[warp][e] - top));
+    for (int e = lane; e < g.E; e += 32) total += expf(static_cast<float>(moe_logit(c.key[warp][e]) - top));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) c.top[warp] = top, c.total[warp] = total;
   }
-  for (int p = threadIdx.x; p < tokens * g.E; p += moe::THREADS) {
+  const int parts = pairs < moe::THREADS ? min(g.E, moe::THREADS / pairs) : 1;
+  for (int w = threadIdx.x; w < pairs * parts; w += moe::THREADS) {
+    const int part = w / pairs, p = w - part * pairs;
     const int tl = p / g.E, e = p - tl * g.E;
-    const double me = isnan(c.v[tl][e]) ? -INFINITY : c.v[tl][e];
-    int place = 0;
-#pragma unroll 8
-    for (int o = 0; o < g.E; ++o) {
-      const double other = c.v[tl][o];
-      place += other > me || (o < e && !(other < me) && (other == me || me == -INFINITY)) ? 1 : 0;
+    const long long* key = c.key[tl];
+    const long long me = key[e];
+    int before = 0;
+    const int o1 = moe_part(g.E, part + 1, parts);
+#pragma unroll 4
+    for (int o = moe_part(g.E, part, parts); o < o1; ++o) before += (o < e ? key[o] >= me : key[o] > me) ? 1 : 0;
+    if (parts == 1)
+      c.place[tl][e] = before;
+    else if (before)
+      atomicAdd(&c.place[tl][e], before);
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < pairs; p += moe::THREADS) {
+    const int tl = p / g.E, e = p - tl * g.E;
+    const int place = c.place[tl][e];
+    if (place < g.top_k) {
+      c.chosen[tl][place] = static_cast<short>(e);
+      c.p[tl][place] = expf(static_cast<float>(moe_logit(c.key[tl][e]) - c.top[tl])) / c.total[tl];
     }
-    if (place < g.top_k) c.chosen[tl][place] = static_cast<short>(e);
   }
   __syncthreads();
   for (int p = threadIdx.x; p < tokens * g.top_k; p += moe::THREADS) {
     const int tl = p / g.top_k, j = p - tl * g.top_k;
-    const double top = c.top[tl];
-    const float total = c.total[tl];
-    float sum = 0.f, mine_p = 0.f;
-    for (int o = 0; o < g.top_k; ++o) {
-      const float pr = expf(static_cast<float>(c.v[tl][c.chosen[tl][o]] - top)) / total;
-      sum += pr;
-      if (o == j) mine_p = pr;
-    }
-    const float coef = g.renorm ? mine_p / sum : mine_p;
+    float sum = 0.f;
+    for (int o = 0; o < g.top_k; ++o) sum += c.p[tl][o];
+    const float coef = g.renorm ? c.p[tl][j] / sum : c.p[tl][j];
     const int at = (rank + tl * moe::CLUSTER) * g.top_k + j;
 #pragma unroll
     for (int d = 0; d < moe::CLUSTER; ++d) {
@@ -470,9 +505,20 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   const int rank = static_cast<int>(rla_cluster_ctarank());
 
   MoeRing ring(rings, sm, warp, lane, stages);
-  if (threadIdx.x == 0) r.abort_flag = 0;
+  if (threadIdx.x == 0) {
+    r.abort_flag = 0;
+    rla_tma_prefetch_desc(&gate_map);
+    rla_tma_prefetch_desc(&up_map);
+  }
+  if (threadIdx.x < moe::MAX_E) r.mask[threadIdx.x] = 0;
   rla_fence_barrier_init();
   rla_griddep_launch_dependents();
+  {  // this CTA's part of the router into L2 while the previous kernel finishes
+    const int64_t lines = ((int64_t)g.E * g.H * 2 + 127) / 128;
+    const char* p = reinterpret_cast<const char*>(g.router);
+    for (int64_t i = rank * moe::THREADS + threadIdx.x; i < lines; i += moe::CLUSTER * moe::THREADS)
+      rla_prefetch_l2(p + i * 128);
+  }
   rla_griddep_wait();
 
   // routing; its scratch lies in the ring, which is not in use yet
@@ -487,23 +533,18 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   moe_choose(g, rank, logits, choose, r);
   rla_cluster_sync();
   rla_fence_proxy_async();  // plain accesses to the ring come before the copies into it
-  if (blockIdx.x == 0)
-    for (int p = threadIdx.x; p < g.T * g.top_k; p += moe::THREADS) {
-      g.ids[p] = r.ids[p];
-      g.coef[p] = r.coef[p];
-    }
   moe_build_lists(r, g.T, g.E, g.top_k);
 
   // This CTA's units, and of their stages this warp's run.
   const int groups = g.I / 8;
   const int per = (g.H + moe::KB - 1) / moe::KB;  // stages of a unit
-  const int64_t units = (int64_t)r.num_active * groups;
-  const int u0 = static_cast<int>(units * blockIdx.x / gridDim.x);
-  const int64_t items = (units * (blockIdx.x + 1) / gridDim.x - u0) * per;
-  const int64_t i0 = items * warp / moe::WARPS;
-  int left = static_cast<int>(items * (warp + 1) / moe::WARPS - i0);
-  const int unit = u0 + static_cast<int>(i0 / per);
-  int ca = unit / groups, cg = unit % groups, cs = static_cast<int>(i0 % per);  // the products' place
+  const int units = r.num_active * groups;
+  const int u0 = moe_part(units, blockIdx.x, gridDim.x);
+  const int items = (moe_part(units, blockIdx.x + 1, gridDim.x) - u0) * per;
+  const int i0 = moe_part(items, warp, moe::WARPS);
+  int left = moe_part(items, warp + 1, moe::WARPS) - i0;
+  const int unit = u0 + i0 / per;
+  int ca = unit / groups, cg = unit % groups, cs = i0 % per;  // the products' place
 
   int pa = ca, pg = cg, ps = cs, to_put = left;  // the copies' place
   int prow = to_put > 0 ? r.active[pa] * g.I + pg * 8 : 0;
@@ -521,6 +562,11 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
     }
   };
   for (int i = 0; i < stages; ++i) put();
+  if (blockIdx.x == 0) {  // for the second kernel
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(static_cast<MoeTables*>(&r));
+    uint32_t* to = reinterpret_cast<uint32_t*>(g.tables);
+    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 4); i += moe::THREADS) to[i] = from[i];
+  }
 
   bool head = left > 0 && cs != 0;  // the current unit began in an earlier warp
   bool tail = false, ok = true;
@@ -560,9 +606,9 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   if (!ok) ring.drain();
   __syncthreads();
   if (tail && ok) {
-    const int64_t end = ((int64_t)ca * groups + cg - u0 + 1) * per;  // the unit's last stage + 1
+    const int end = (ca * groups + cg - u0 + 1) * per;  // the unit's last stage + 1
     for (int w = warp + 1; w < moe::WARPS; ++w) {
-      const int64_t w0 = items * w / moe::WARPS, w1 = items * (w + 1) / moe::WARPS;
+      const int w0 = moe_part(items, w, moe::WARPS), w1 = moe_part(items, w + 1, moe::WARPS);
       if (w0 >= end) break;
       if (w0 == w1) continue;
       const float* h = heads + w * NT * 128 + lane;
@@ -591,23 +637,26 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_
   const int splits = gridDim.y, split = blockIdx.y;  // == cluster rank
 
   MoeRing ring(smem + moe_ring_offset(g.T), sm, warp, lane, stages);
-  if (threadIdx.x == 0) r.abort_flag = 0;
+  if (threadIdx.x == 0) {
+    r.abort_flag = 0;
+    rla_tma_prefetch_desc(&down_map);
+  }
   rla_fence_barrier_init();
   rla_griddep_launch_dependents();
   rla_griddep_wait();
-  for (int p = threadIdx.x; p < g.T * g.top_k; p += moe::THREADS) {
-    r.ids[p] = g.ids[p];
-    r.coef[p] = g.coef[p];
+  {
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(g.tables);
+    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<MoeTables*>(&r));
+    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 4); i += moe::THREADS) to[i] = __ldcg(from + i);
   }
   __syncthreads();
-  moe_build_lists(r, g.T, g.E, g.top_k);
 
   const int blocks = g.H / 16;
   const int per = (g.I + moe::KB - 1) / moe::KB;
-  const int64_t items = (int64_t)r.num_active * per;
+  const int items = r.num_active * per;
   const int parts = splits * moe::WARPS, mine = split * moe::WARPS + warp;
-  const int i0 = static_cast<int>(items * mine / parts), n = static_cast<int>(items * (mine + 1) / parts) - i0;
-  const int a0 = i0 / per, s0 = i0 % per;
+  const int i0 = moe_part(items, mine, parts), n = moe_part(items, mine + 1, parts) - i0;
+  const int a0 = i0 / per, s0 = i0 - a0 * per;
 
   // the copies run through all blocks of this CTA without a break
   int pb = blockIdx.x, pa = a0, ps = s0, pi = 0;
@@ -771,7 +820,7 @@ extern "C" {
 size_t rla_moe_workspace_size(int64_t T, int64_t I, int64_t top_k) {
   if (T <= 0 || I <= 0 || top_k <= 0 || T > RLA_MOE_MAX_TOKENS || top_k > RLA_MOE_MAX_TOP_K) return 0;
   const size_t n = (size_t)T * (size_t)top_k;
-  return rla::moe_up256(n * (size_t)I * 2) + 2 * rla::moe_up256(n * 4);
+  return rla::moe_up256(n * (size_t)I * 2) + rla::moe_up256(sizeof(rla::MoeTables));
 }
 
 int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate, const void* scale_gate,
@@ -781,8 +830,8 @@ int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate
   using namespace rla;
   static_assert(moe::MAX_T == RLA_MOE_MAX_TOKENS && moe::MAX_E == RLA_MOE_MAX_EXPERTS && moe::MAX_K == RLA_MOE_MAX_TOP_K,
                 "limits of the header");
-  if (T < 0 || H < 1 || I < 1 || E < 1 || H > (1 << 20) || I > (1 << 20))
-    return moe_fail(RLA_ERR_INVALID_ARGUMENT, "T must be >= 0, H and I in [1, 2^20], E >= 1");
+  if (T < 0 || H < 1 || I < 1 || E < 1 || H > (1 << 17) || I > (1 << 17))
+    return moe_fail(RLA_ERR_INVALID_ARGUMENT, "T must be >= 0, H and I in [1, 2^17], E >= 1");
   if (top_k < 1 || top_k > E) return moe_fail(RLA_ERR_INVALID_ARGUMENT, "top_k must be in [1, E]");
   if (T > moe::MAX_T || E > moe::MAX_E || top_k > moe::MAX_K)
     return moe_fail(RLA_ERR_UNSUPPORTED, "at most 32 tokens, 256 experts and top_k 32");
@@ -807,8 +856,7 @@ int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate
   const size_t a_bytes = moe_up256(n * (size_t)I * 2);
   const MoeArgs g{static_cast<const __half*>(x), ldx, static_cast<const __half*>(router), w_gate, w_up, w_down,
                   scale_gate, scale_up, scale_down, scale_dtype == RLA_DTYPE_F32 ? 1 : 0, static_cast<__half*>(y), ldy,
-                  reinterpret_cast<__half*>(ws), reinterpret_cast<int*>(ws + a_bytes),
-                  reinterpret_cast<float*>(ws + a_bytes + moe_up256(n * 4)), (int)T, (int)H, (int)I, (int)E, (int)top_k,
+                  reinterpret_cast<__half*>(ws), reinterpret_cast<MoeTables*>(ws + a_bytes), (int)T, (int)H, (int)I, (int)E, (int)top_k,
                   renormalize ? 1 : 0};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = moe_tiles((int)T) == 1   ? launch_moe<1>(g, s)

@@ -119,6 +119,7 @@ def test_capi_rejects_bad_arguments(lib):
     assert moe(k=0) == 1 and moe(k=9) == 1
     assert moe(T=33) == 2 and moe(E=257) == 2 and moe(E=64, k=33) == 2
     assert moe(H=72, ldx=72, ldy=72) == 2 and moe(I=40) == 2
+    assert moe(H=1 << 18, ldx=1 << 18, ldy=1 << 18) == 1 and moe(I=1 << 18) == 1
     assert moe(sdt=0) == 1 and moe(sdt=3) == 1
     for name in ("x", "r", "wg", "sg", "wu", "su", "wd", "sd", "y"):
         assert moe(**{name: None}) == 1
@@ -126,7 +127,7 @@ def test_capi_rejects_bad_arguments(lib):
     assert moe(x=odd) == 2 and moe(r=odd) == 2 and moe(wg=odd) == 2 and moe(wu=odd) == 2 and moe(wd=odd) == 2
     assert moe(ldx=68) == 2
     need = lib.rla_moe_workspace_size(4, 32, 2)
-    assert need == 512 + 256 + 256
+    assert need >= 4 * 2 * 32 * 2 and need % 256 == 0      # fp16 activations of 8 (token, expert) pairs, and the routing
     assert moe(ws=None) == 4 and moe(wsb=need - 1) == 4 and moe(ws=ctypes.c_void_p(4096 + 128)) == 4
     assert b"workspace" in lib.rla_last_error()
     assert moe(T=0) == 0
