@@ -28,9 +28,9 @@
 //
 // Routing.  Which weights to read is not known before the logits are, so
 // the whole GPU waits for them.  Each cluster of 4 CTAs computes all logits by
-// itself (K split over its CTAs, joined through distributed shared memory):
-// no grid-wide barrier, one kernel launch less, and 1/4 of the router's bytes
-// an SM.  A choice between two experts is a border, so the partial logits
+// itself (K split over its CTAs, joined through distributed shared memory),
+// and each CTA makes all choices for itself: no grid-wide barrier, one kernel
+// launch less, and 1/4 of the router's bytes an SM.  A choice between two experts is a border, so the partial logits
 // (fp32 sums over 1/4 of K or less) are added in 64 bits.  Ties go to the
 // lower index.
 //
@@ -73,7 +73,7 @@ struct MoeTables {
   short active[moe::MAX_E];             // experts that some token chose, in order
   short entry[moe::MAX_T * moe::MAX_K];
   uint8_t token[moe::MAX_T * moe::MAX_K];
-  int num_active;
+  int num_active, unused[3];  // (a multiple of 16 bytes)
 };
 
 struct MoeArgs {
@@ -97,10 +97,6 @@ struct MoeArgs {
 RLA_DEVFN float moe_scale(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : __half2float(static_cast<const __half*>(p)[i]);
 }
-// Store into CTA `rank`'s copy of the shared variable at `p`.
-RLA_DEVFN void rla_st_dsmem_u32(const void* p, uint32_t rank, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(rla_mapa(rla_smem_u32(p), rank)), "r"(v) : "memory");
-}
 RLA_DEVFN double rla_ld_dsmem_f64(const void* p, uint32_t rank) {
   double v;
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(rla_mapa(rla_smem_u32(p), rank)) : "memory");
@@ -110,6 +106,15 @@ RLA_DEVFN float rla_ld_dsmem_f32(const void* p, uint32_t rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(rla_mapa(rla_smem_u32(p), rank)) : "memory");
   return v;
+}
+// The two halves of rla_cluster_sync.
+RLA_DEVFN void rla_cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+RLA_DEVFN void rla_cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 RLA_DEVFN uint4 rla_lds128(uint32_t addr) {
   uint4 v;
@@ -192,10 +197,9 @@ struct MoeRing {
   }
 };
 
-// ids -> mask (zero before), begin, active, entry, token.  All threads of the CTA.
+// ids, mask -> begin, active, entry, token.  All threads of the CTA.
 RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
   const int tid = threadIdx.x, lane = tid & 31;
-  for (int p = tid; p < T * top_k; p += moe::THREADS) atomicOr(&r.mask[r.ids[p]], 1u << (p / top_k));
   __syncthreads();
   if (tid < 32) {  // a lane takes PER experts in a row
     constexpr int PER = moe::MAX_E / 32;
@@ -246,33 +250,44 @@ RLA_DEVFN int moe_part(int total, int i, int n) {
 // different halves of the 32 banks.
 RLA_DEVFN int moe_row(int g) { return (g >> 1) | ((g & 1) << 2); }
 
-// One stage: 16 weight rows x up to 256 k (four 64-wide chunks) in shared
-// memory at `w` times NT tiles of 8 columns.  xp[t]: this lane's activations of column 8 t + lane / 4 at
-// the stage's first k + 16 * (lane % 4).  The k order inside the fragments
-// follows the 16-byte pieces (rla_skinny.cu).  FULL: all 256 k are there;
-// otherwise `bytes` are, and behind them zeros meet zeros or stale, finite weights.
-template <int NT, bool FULL>
-RLA_DEVFN void moe_stage(float (&acc)[4][4], uint32_t w, const __half* const (&xp)[NT], int bytes, int lane) {
-  const int q = lane & 3;
-  constexpr int CHUNKS = moe::KB / 64;
-  const int row = moe_row(lane >> 2);
-  // 16-byte pieces q and 4 + q of the row (the 64-wide chunks of a half)
-  const uint32_t w0_at = w + row * 128 + ((q ^ row) << 4), w1_at = w + row * 128 + (((4 + q) ^ row) << 4);
-  constexpr int AHEAD = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks of activations held in registers
-  uint4 xb[AHEAD][NT][2];
-  auto load = [&](int c) {
+// Activations of one stage.  xp[t]: this lane's of column 8 t + lane / 4 at
+// the stage's first k + 16 * (lane % 4); load(c) reads those of the 64-wide
+// chunk c.  The k order inside the fragments follows the 16-byte pieces
+// (rla_skinny.cu).  FULL: all 256 k are there; otherwise `bytes` are, and
+// behind them zeros meet zeros or stale, finite weights.
+template <int NT>
+struct MoeActs {
+  static constexpr int AHEAD = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks held in registers
+  uint4 v[AHEAD][NT][2];
+  template <bool FULL>
+  RLA_DEVFN void load(int c, const __half* const (&xp)[NT], int bytes, int q) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (FULL || c * 64 + q * 16 < bytes) {
-        xb[c % AHEAD][t][0] = rla_ldg_keep(xp[t] + c * 64);
-        xb[c % AHEAD][t][1] = rla_ldg_keep(xp[t] + c * 64 + 8);
+        v[c % AHEAD][t][0] = rla_ldg_keep(xp[t] + c * 64);
+        v[c % AHEAD][t][1] = rla_ldg_keep(xp[t] + c * 64 + 8);
       } else {
-        xb[c % AHEAD][t][0] = xb[c % AHEAD][t][1] = make_uint4(0, 0, 0, 0);
+        v[c % AHEAD][t][0] = v[c % AHEAD][t][1] = make_uint4(0, 0, 0, 0);
       }
     }
-  };
+  }
+};
+
+// One stage from the ring: 16 weight rows x up to 256 k (four chunks) times NT
+// tiles of 8 columns.  The first activations are on their way before the wait.
+template <int NT, bool FULL>
+RLA_DEVFN bool moe_stage(float (&acc)[4][4], MoeRing& ring, const __half* const (&xp)[NT], int bytes, int lane,
+                         volatile int* abort_flag) {
+  const int q = lane & 3;
+  constexpr int CHUNKS = moe::KB / 64;
+  MoeActs<NT> x;
 #pragma unroll
-  for (int c = 0; c < AHEAD; ++c) load(c);
+  for (int c = 0; c < x.AHEAD; ++c) x.template load<FULL>(c, xp, bytes, q);
+  uint32_t w;
+  if (!ring.wait(abort_flag, w)) return false;
+  const int row = moe_row(lane >> 2);
+  // 16-byte pieces q and 4 + q of the row (the 64-wide chunks of a half)
+  const uint32_t w0_at = w + row * 128 + ((q ^ row) << 4), w1_at = w + row * 128 + (((4 + q) ^ row) << 4);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const uint32_t at = (c & 1 ? w1_at : w0_at) + (c >> 1) * moe::HALF;
@@ -286,12 +301,13 @@ RLA_DEVFN void moe_stage(float (&acc)[4][4], uint32_t w, const __half* const (&x
       rla_i8x4_to_h2x2(w1[s], a1, a3);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const uint32_t* xw = reinterpret_cast<const uint32_t*>(&xb[c % AHEAD][t][0]);
+        const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x.v[c % x.AHEAD][t][0]);
         rla_mma_16816(acc[t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
       }
     }
-    if (c + AHEAD < CHUNKS) load(c + AHEAD);
+    if (c + x.AHEAD < CHUNKS) x.template load<FULL>(c + x.AHEAD, xp, bytes, q);
   }
+  return true;
 }
 
 // `n` stages of one expert from the ring, from k = k0 of `width` on.  Columns
@@ -307,13 +323,10 @@ RLA_DEVFN bool moe_run_tiles(float (&acc)[4][4], MoeRing& ring, int n, int k0, i
     xp[t] = row(col < count ? col : 0) + k0 + (lane & 3) * 16;
   }
   for (int i = 0; i < n; ++i) {
-    uint32_t at;
-    if (!ring.wait(abort_flag, at)) return false;
     const int bytes = width - k0 - i * moe::KB;
-    if (bytes >= moe::KB)
-      moe_stage<NT, true>(acc, at, xp, bytes, lane);
-    else
-      moe_stage<NT, false>(acc, at, xp, bytes, lane);
+    if (!(bytes >= moe::KB ? moe_stage<NT, true>(acc, ring, xp, bytes, lane, abort_flag)
+                           : moe_stage<NT, false>(acc, ring, xp, bytes, lane, abort_flag)))
+      return false;
     __syncwarp();
     put();
 #pragma unroll
@@ -378,24 +391,13 @@ RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part, double* v) {
   __syncthreads();
   for (int p = threadIdx.x; p < g.T * g.E; p += moe::THREADS) {
     double sum = 0;
+#pragma unroll 4
     for (int j = 0; j < parts; ++j) sum += static_cast<double>(part[j * g.T * g.E + p]);
     v[p] = sum;
   }
 }
 
-// Softmax and choice of the tokens t = rank, rank + CLUSTER, ..., from all
-// ranks' partial logits; ids and coef go into every CTA of the cluster.  An
-// expert's place is the number of experts before it (larger logit, or equal
-// and a lower index), counted by all threads at once; a NaN counts as the
-// smallest, so that every place is taken.
-struct MoeChoose {
-  long long key[moe::MAX_T / moe::CLUSTER][moe::MAX_E];  // the logits as integers of the same order
-  int place[moe::MAX_T / moe::CLUSTER][moe::MAX_E];
-  double top[moe::MAX_T / moe::CLUSTER];
-  float total[moe::MAX_T / moe::CLUSTER];
-  short chosen[moe::MAX_T / moe::CLUSTER][moe::MAX_K];
-  float p[moe::MAX_T / moe::CLUSTER][moe::MAX_K];
-};
+// A logit as an integer of the same order; a NaN counts as the smallest.
 RLA_DEVFN long long moe_key(double v) {  // (never -0: sums start from +0)
   const long long b = __double_as_longlong(v);
   return isnan(v) ? LLONG_MIN : b >= 0 ? b : b ^ LLONG_MAX;
@@ -403,72 +405,77 @@ RLA_DEVFN long long moe_key(double v) {  // (never -0: sums start from +0)
 RLA_DEVFN double moe_logit(long long key) {
   return key == LLONG_MIN ? __longlong_as_double(LLONG_MAX) : __longlong_as_double(key >= 0 ? key : key ^ LLONG_MAX);
 }
-RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, const double* mine, MoeChoose& c, MoeRoute& r) {
+
+// Softmax and choice from all ranks' partial logits: a warp a token, every
+// CTA of the cluster for itself.  top_k rounds of "the largest that is left,
+// the lowest index of equals"; every round finds an expert, NaN or not.
+template <int PER>  // experts of a lane, at least E / 32
+RLA_DEVFN void moe_choose_of(const MoeArgs& g, const double* mine, MoeRoute& r) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tokens = g.T > rank ? (g.T - rank + moe::CLUSTER - 1) / moe::CLUSTER : 0;
-  const int pairs = tokens * g.E;
-  if (pairs == 0) return;  // (the whole CTA)
-  for (int p = threadIdx.x; p < pairs; p += moe::THREADS) {
-    const int tl = p / g.E, e = p - tl * g.E;
-    double part[moe::CLUSTER], sum = 0;
+  for (int t = warp; t < g.T; t += moe::WARPS) {
+    double part[PER][moe::CLUSTER];
 #pragma unroll
-    for (int d = 0; d < moe::CLUSTER; ++d)
-      part[d] = rla_ld_dsmem_f64(mine + (rank + tl * moe::CLUSTER) * g.E + e, d);
+    for (int i = 0; i < PER; ++i)
 #pragma unroll
-    for (int d = 0; d < moe::CLUSTER; ++d) sum += part[d];
-    c.key[tl][e] = moe_key(sum);
-    c.place[tl][e] = 0;
-  }
-  __syncthreads();
-  static_assert(moe::WARPS >= moe::MAX_T / moe::CLUSTER, "a warp a token");
-  if (warp < tokens) {
-    double top = -INFINITY;
-    for (int e = lane; e < g.E; e += 32) top = fmax(top, moe_logit(c.key[warp][e]));  // (drops NaN)
+      for (int d = 0; d < moe::CLUSTER; ++d)  // (a lane without an expert repeats the last one)
+        part[i][d] = rla_ld_dsmem_f64(mine + t * g.E + min(i * 32 + lane, g.E - 1), d);
+    long long key[PER];
+    uint32_t left = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float total = 0.f;  // a NaN logit makes it NaN
-    for (int e = lane; e < g.E; e += 32) total += expf(static_cast<float>(moe_logit(c.key[warp][e]) - top));
+    for (int i = 0; i < PER; ++i) {
+      double sum = 0;
+#pragma unroll
+      for (int d = 0; d < moe::CLUSTER; ++d) sum += part[i][d];
+      key[i] = moe_key(sum);
+      left |= i * 32 + lane < g.E ? 1u << i : 0u;
+    }
+    int my_id = 0;
+    long long my_key = 0;
+    double top = 0;
+    uint32_t taken = 0;
+    for (int j = 0; j < g.top_k; ++j) {
+      long long best = LLONG_MIN;
+      unsigned at = 0xffffffffu;  // none left in this lane
+#pragma unroll
+      for (int i = PER - 1; i >= 0; --i)
+        if ((left & ~taken) >> i & 1 && key[i] >= best) best = key[i], at = i * 32 + lane;
+      const int hi = static_cast<int>(best >> 32);
+      const int hi_max = __reduce_max_sync(0xffffffffu, hi);
+      const unsigned lo = hi == hi_max ? static_cast<unsigned>(best) : 0u;
+      const unsigned lo_max = __reduce_max_sync(0xffffffffu, lo);
+      const unsigned e = __reduce_min_sync(0xffffffffu, hi == hi_max && lo == lo_max ? at : 0xffffffffu);
+      if (lane == (e & 31)) taken |= 1u << (e >> 5);
+      const long long k = static_cast<long long>(static_cast<unsigned long long>(static_cast<unsigned>(hi_max)) << 32 | lo_max);
+      if (j == 0) top = moe_logit(k);
+      if (lane == j) my_id = static_cast<int>(e), my_key = k;
+    }
+    // softmax relative to the largest; a NaN logit makes the sum NaN
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (left >> i & 1) total += expf(static_cast<float>(moe_logit(key[i]) - top));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) c.top[warp] = top, c.total[warp] = total;
-  }
-  const int parts = pairs < moe::THREADS ? min(g.E, moe::THREADS / pairs) : 1;
-  for (int w = threadIdx.x; w < pairs * parts; w += moe::THREADS) {
-    const int part = w / pairs, p = w - part * pairs;
-    const int tl = p / g.E, e = p - tl * g.E;
-    const long long* key = c.key[tl];
-    const long long me = key[e];
-    int before = 0;
-    const int o1 = moe_part(g.E, part + 1, parts);
-#pragma unroll 4
-    for (int o = moe_part(g.E, part, parts); o < o1; ++o) before += (o < e ? key[o] >= me : key[o] > me) ? 1 : 0;
-    if (parts == 1)
-      c.place[tl][e] = before;
-    else if (before)
-      atomicAdd(&c.place[tl][e], before);
-  }
-  __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += moe::THREADS) {
-    const int tl = p / g.E, e = p - tl * g.E;
-    const int place = c.place[tl][e];
-    if (place < g.top_k) {
-      c.chosen[tl][place] = static_cast<short>(e);
-      c.p[tl][place] = expf(static_cast<float>(moe_logit(c.key[tl][e]) - c.top[tl])) / c.total[tl];
-    }
-  }
-  __syncthreads();
-  for (int p = threadIdx.x; p < tokens * g.top_k; p += moe::THREADS) {
-    const int tl = p / g.top_k, j = p - tl * g.top_k;
-    float sum = 0.f;
-    for (int o = 0; o < g.top_k; ++o) sum += c.p[tl][o];
-    const float coef = g.renorm ? c.p[tl][j] / sum : c.p[tl][j];
-    const int at = (rank + tl * moe::CLUSTER) * g.top_k + j;
+    const float p = lane < g.top_k ? expf(static_cast<float>(moe_logit(my_key) - top)) / total : 0.f;
+    float chosen = p;
 #pragma unroll
-    for (int d = 0; d < moe::CLUSTER; ++d) {
-      rla_st_dsmem_u32(&r.ids[at], d, static_cast<uint32_t>(c.chosen[tl][j]));
-      rla_st_dsmem_u32(&r.coef[at], d, __float_as_uint(coef));
+    for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
+    if (lane < g.top_k) {
+      r.ids[t * g.top_k + lane] = my_id;
+      r.coef[t * g.top_k + lane] = g.renorm ? p / chosen : p;
+      atomicOr(&r.mask[my_id], 1u << t);
     }
   }
+}
+RLA_DEVFN void moe_choose(const MoeArgs& g, const double* mine, MoeRoute& r) {
+  if (g.E <= 32)
+    moe_choose_of<1>(g, mine, r);
+  else if (g.E <= 64)
+    moe_choose_of<2>(g, mine, r);
+  else if (g.E <= 128)
+    moe_choose_of<4>(g, mine, r);
+  else
+    moe_choose_of<8>(g, mine, r);
 }
 
 // A unit of the gate/up kernel: 8 gate rows and the same 8 up rows of one expert.
@@ -524,16 +531,16 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   // routing; its scratch lies in the ring, which is not in use yet
   constexpr int PART = moe::WARPS * 16 * 8 * NT * 4;  // [parts][T][E] floats at most
   constexpr int LOGITS = 8 * NT * moe::MAX_E * 8;
-  static_assert(PART + LOGITS + sizeof(MoeChoose) <= moe::WARPS * 2 * moe::SLOT, "routing scratch fits the ring");
+  static_assert(PART + LOGITS <= moe::WARPS * 2 * moe::SLOT, "routing scratch fits the ring");
   float* part = reinterpret_cast<float*>(rings);
   double* logits = reinterpret_cast<double*>(rings + PART);
-  MoeChoose& choose = *reinterpret_cast<MoeChoose*>(rings + PART + LOGITS);
   moe_logits<NT>(g, rank, part, logits);
   rla_cluster_sync();
-  moe_choose(g, rank, logits, choose, r);
-  rla_cluster_sync();
-  rla_fence_proxy_async();  // plain accesses to the ring come before the copies into it
+  moe_choose(g, logits, r);
+  rla_cluster_arrive();  // this CTA has read the others' logits ...
   moe_build_lists(r, g.T, g.E, g.top_k);
+  rla_cluster_wait();    // ... and the others this one's: the ring is free
+  rla_fence_proxy_async();  // plain accesses to the ring come before the copies into it
 
   // This CTA's units, and of their stages this warp's run.
   const int groups = g.I / 8;
@@ -563,9 +570,9 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   };
   for (int i = 0; i < stages; ++i) put();
   if (blockIdx.x == 0) {  // for the second kernel
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(static_cast<MoeTables*>(&r));
-    uint32_t* to = reinterpret_cast<uint32_t*>(g.tables);
-    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 4); i += moe::THREADS) to[i] = from[i];
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<MoeTables*>(&r));
+    uint4* to = reinterpret_cast<uint4*>(g.tables);
+    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 16); i += moe::THREADS) to[i] = from[i];
   }
 
   bool head = left > 0 && cs != 0;  // the current unit began in an earlier warp
@@ -645,9 +652,11 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_
   rla_griddep_launch_dependents();
   rla_griddep_wait();
   {
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(g.tables);
-    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<MoeTables*>(&r));
-    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 4); i += moe::THREADS) to[i] = __ldcg(from + i);
+    const uint4* from = reinterpret_cast<const uint4*>(g.tables);
+    uint4* to = reinterpret_cast<uint4*>(static_cast<MoeTables*>(&r));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(MoeTables) / 16); i += moe::THREADS)
+      if (i + threadIdx.x < sizeof(MoeTables) / 16) to[i + threadIdx.x] = __ldcg(from + i + threadIdx.x);
   }
   __syncthreads();
 
