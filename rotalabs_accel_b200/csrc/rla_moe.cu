@@ -9,9 +9,9 @@
 // read once, by one warp, and meets all tokens that chose its expert.
 //
 // Stream.  Every warp has a ring of its own in shared memory, filled by bulk
-// tile copies that it issues itself: a stage is 256 bytes of 16 weight rows,
-// in two or four copies.  (One copy a row cost 16 issues, a third of all
-// instructions: 93 us for the case below.)  One CTA of 16 warps an SM keeps 16 x STAGES x 4 KB on their way
+// tile copies that it issues itself: a stage is 128 bytes of 32 weight rows,
+// in one or two copies.  (One copy a row cost 16 issues, a third of all
+// instructions: 93 us for the case below.)  One CTA of 12 or 16 warps an SM keeps warps x stages x 4 KB on their way
 // (latency x bandwidth needs about 50 KB), through every reduction and change
 // of expert, and no warp waits for another one's data.  (Loads into registers,
 // with the warps of a CTA splitting K and meeting after every 16 rows, took
@@ -47,18 +47,21 @@
 namespace rla {
 
 namespace moe {
-constexpr int WARPS = 16;
-constexpr int THREADS = 32 * WARPS;
+// By the tiles of 8 tokens (NT = 1, 2, 4): more accumulators, fewer warps, so
+// that nothing spills (a spilled register comes back from an L2 that is busy
+// with weights, microseconds later).
+__host__ __device__ constexpr int warps(int nt) { return nt == 4 ? 12 : 16; }
+constexpr int MAX_WARPS = 16;
 constexpr int CLUSTER = 4;
 constexpr int MAX_T = 32;
 constexpr int MAX_E = 256;
 constexpr int MAX_K = 32;  // top_k
 constexpr int MAX_SPLITS = 8;
-constexpr int KB = 256;  // bytes of a weight row in a stage: four 64-wide chunks
-// A stage is two halves of 128 bytes x 16 rows, 128-byte swizzled by the copy
-// (16-byte piece c of row r lies at piece c ^ (r % 8)).
-constexpr int HALF = 16 * 128;
-constexpr int SLOT = 16 * KB;
+// A stage: 128 bytes of 32 weight rows (two 64-wide chunks), 128-byte swizzled
+// by the copy (16-byte piece c of row r lies at piece c ^ (r % 8)).
+constexpr int KB = 128;
+constexpr int ROWS = 32;
+constexpr int SLOT = ROWS * KB;
 constexpr int MAX_STAGES = 3;
 constexpr size_t SMEM = 227 * 1024;  // of a CTA
 }  // namespace moe
@@ -128,16 +131,16 @@ struct MoeRoute : MoeTables {
 };
 
 // Shared memory of both kernels: routing, barriers, a buffer for partial sums
-// (16 warps x 16 values for each column of the 8-token tiles), the warps' rings.
+// (warps x 32 values for each column of the 8-token tiles), the warps' rings.
 struct MoeShared {
   MoeRoute r;
-  uint64_t full[moe::WARPS][moe::MAX_STAGES];
+  uint64_t full[moe::MAX_WARPS][moe::MAX_STAGES];
 };
 __host__ __device__ constexpr size_t moe_sums_offset() { return (sizeof(MoeShared) + 1023) & ~size_t(1023); }
 __host__ __device__ constexpr int moe_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
-__host__ __device__ constexpr size_t moe_ring_offset(int T) { return moe_sums_offset() + (size_t)moe_tiles(T) * 8192; }
+__host__ __device__ constexpr size_t moe_ring_offset(int T) { return moe_sums_offset() + (size_t)moe_tiles(T) * moe::warps(moe_tiles(T)) * 1024; }
 __host__ __device__ constexpr size_t moe_smem_bytes(int T, int stages) {
-  return 1024 + moe_ring_offset(T) + (size_t)moe::WARPS * stages * moe::SLOT;
+  return 1024 + moe_ring_offset(T) + (size_t)moe::warps(moe_tiles(T)) * stages * moe::SLOT;
 }
 
 // A warp's ring: issue() starts the copy of the next stage, wait() waits for
@@ -152,21 +155,16 @@ struct MoeRing {
     full = sm.full[warp];
     if (lane < n) rla_mbar_init(&full[lane], 1);
   }
-  // The next stage: columns [k, k + 256) of 16 rows, rows r0.. of map0 (all 16,
-  // or 8 of them and rows r0.. of map1).
+  // The next stage: columns [k, k + 128) of rows r0.. of map0 (all 32, or 16
+  // of them and the same 16 rows of map1).
   template <int MAPS>
-  RLA_DEVFN void issue(const CUtensorMap* map0, const CUtensorMap* map1, int k, int r0, int width, int lane) {
+  RLA_DEVFN void issue(const CUtensorMap* map0, const CUtensorMap* map1, int k, int r0, int lane) {
     if (lane == 0) {
       uint64_t* bar = &full[put_slot];
       const uint32_t to = base + put_slot * moe::SLOT;
-      const int halves = width - k > 128 ? 2 : 1;
-      rla_mbar_arrive_expect_tx(bar, halves * moe::HALF);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == halves) break;
-        tile(to + h * moe::HALF, map0, bar, k + h * 128, r0);
-        if (MAPS == 2) tile(to + h * moe::HALF + 1024, map1, bar, k + h * 128, r0);
-      }
+      rla_mbar_arrive_expect_tx(bar, moe::SLOT);
+      tile(to, map0, bar, k, r0);
+      if (MAPS == 2) tile(to + moe::SLOT / 2, map1, bar, k, r0);
     }
     put_slot = put_slot + 1 == stages ? 0 : put_slot + 1;
     ++flying;
@@ -229,7 +227,7 @@ RLA_DEVFN void moe_build_lists(MoeRoute& r, int T, int E, int top_k) {
     }
   }
   __syncthreads();
-  for (int p = tid; p < T * top_k; p += moe::THREADS) {
+  for (int p = tid; p < T * top_k; p += blockDim.x) {
     const int t = p / top_k, e = r.ids[p];
     const int at = r.begin[e] + __popc(r.mask[e] & ((1u << t) - 1));
     r.entry[at] = static_cast<short>(p);
@@ -250,100 +248,135 @@ RLA_DEVFN int moe_part(int total, int i, int n) {
 // different halves of the 32 banks.
 RLA_DEVFN int moe_row(int g) { return (g >> 1) | ((g & 1) << 2); }
 
-// Activations of one stage.  xp[t]: this lane's of column 8 t + lane / 4 at
-// the stage's first k + 16 * (lane % 4); load(c) reads those of the 64-wide
-// chunk c.  The k order inside the fragments follows the 16-byte pieces
-// (rla_skinny.cu).  FULL: all 256 k are there; otherwise `bytes` are, and
-// behind them zeros meet zeros or stale, finite weights.
+// Activations of a stage.  xp[t]: this lane's of column 8 t + lane / 4 at the
+// stage's first k + 16 * (lane % 4); load(c) reads those of the 64-wide chunk
+// c.  The k order inside the fragments follows the 16-byte pieces
+// (rla_skinny.cu).  `bytes`: the k that are left; behind them zeros meet zeros.
 template <int NT>
 struct MoeActs {
-  static constexpr int AHEAD = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks held in registers
-  uint4 v[AHEAD][NT][2];
+  static constexpr int HELD = NT <= 2 ? 2 : 1;  // chunks in registers
+  uint4 v[HELD][NT][2];
   template <bool FULL>
   RLA_DEVFN void load(int c, const __half* const (&xp)[NT], int bytes, int q) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (FULL || c * 64 + q * 16 < bytes) {
-        v[c % AHEAD][t][0] = rla_ldg_keep(xp[t] + c * 64);
-        v[c % AHEAD][t][1] = rla_ldg_keep(xp[t] + c * 64 + 8);
+        v[c % HELD][t][0] = rla_ldg_keep(xp[t] + c * 64);
+        v[c % HELD][t][1] = rla_ldg_keep(xp[t] + c * 64 + 8);
       } else {
-        v[c % AHEAD][t][0] = v[c % AHEAD][t][1] = make_uint4(0, 0, 0, 0);
+        v[c % HELD][t][0] = v[c % HELD][t][1] = make_uint4(0, 0, 0, 0);
       }
+    }
+  }
+  RLA_DEVFN void load_first(const __half* const (&xp)[NT], int bytes, int q) {
+    if (bytes >= moe::KB) {
+#pragma unroll
+      for (int c = 0; c < HELD; ++c) load<true>(c, xp, bytes, q);
+    } else {
+#pragma unroll
+      for (int c = 0; c < HELD; ++c) load<false>(c, xp, bytes, q);
     }
   }
 };
 
-// One stage from the ring: 16 weight rows x up to 256 k (four chunks) times NT
-// tiles of 8 columns.  The first activations are on their way before the wait.
-template <int NT, bool FULL>
-RLA_DEVFN bool moe_stage(float (&acc)[4][4], MoeRing& ring, const __half* const (&xp)[NT], int bytes, int lane,
-                         volatile int* abort_flag) {
+// Two row tiles of 16 x NTM column tiles of 8 (those of all tokens), fp32.
+template <int NTM>
+using MoeAcc = float[2][NTM][4];
+
+// One stage in shared memory at `w`: 32 weight rows x 128 k times NT tiles of
+// 8 columns.  Row g of row tile m is at row m * STEP / 128 + moe_row(g) of the
+// stage, row 8 + g UPPER bytes behind it.  The first chunks of x are loaded.
+template <int NT, int STEP, int UPPER, int NTM>
+RLA_DEVFN void moe_stage(float (&acc)[2][NTM][4], uint32_t w, MoeActs<NT>& x, const __half* const (&xp)[NT], int bytes, int lane) {
   const int q = lane & 3;
-  constexpr int CHUNKS = moe::KB / 64;
-  MoeActs<NT> x;
-#pragma unroll
-  for (int c = 0; c < x.AHEAD; ++c) x.template load<FULL>(c, xp, bytes, q);
-  uint32_t w;
-  if (!ring.wait(abort_flag, w)) return false;
   const int row = moe_row(lane >> 2);
-  // 16-byte pieces q and 4 + q of the row (the 64-wide chunks of a half)
-  const uint32_t w0_at = w + row * 128 + ((q ^ row) << 4), w1_at = w + row * 128 + (((4 + q) ^ row) << 4);
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const uint32_t at = (c & 1 ? w1_at : w0_at) + (c >> 1) * moe::HALF;
-    const uint4 wa = rla_lds128(at), wb = rla_lds128(at + 1024);
-    const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&wa);
-    const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&wb);
+  for (int c = 0; c < 2; ++c) {
+    const uint32_t at = w + row * 128 + (((c * 4 + q) ^ row) << 4);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      uint32_t a0, a1, a2, a3;
-      rla_i8x4_to_h2x2(w0[s], a0, a2);
-      rla_i8x4_to_h2x2(w1[s], a1, a3);
+    for (int m = 0; m < 2; ++m) {
+      const uint4 wa = rla_lds128(at + m * STEP), wb = rla_lds128(at + m * STEP + UPPER);
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&wa);
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&wb);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x.v[c % x.AHEAD][t][0]);
-        rla_mma_16816(acc[t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
+      for (int s = 0; s < 4; ++s) {
+        uint32_t a0, a1, a2, a3;
+        rla_i8x4_to_h2x2(w0[s], a0, a2);
+        rla_i8x4_to_h2x2(w1[s], a1, a3);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x.v[c % x.HELD][t][0]);
+          rla_mma_16816(acc[m][t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
+        }
       }
     }
-    if (c + x.AHEAD < CHUNKS) x.template load<FULL>(c + x.AHEAD, xp, bytes, q);
+    if (c == 0 && x.HELD == 1) {
+      if (bytes >= moe::KB)
+        x.template load<true>(1, xp, bytes, q);
+      else
+        x.template load<false>(1, xp, bytes, q);
+    }
   }
-  return true;
 }
 
 // `n` stages of one expert from the ring, from k = k0 of `width` on.  Columns
 // are the expert's tokens; the columns behind them repeat its first token and
 // are not used.  row(i): the activations' row of the expert's i-th entry.
-template <int NT, class Row, class Put>
-RLA_DEVFN bool moe_run_tiles(float (&acc)[4][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
+//
+// The activations come from L2, whose latency a warp would meet at every
+// stage: up to 8 tokens they are loaded a stage ahead.  32 rows share them
+// (16 rows of 256 bytes a stage needed twice the loads, and too many
+// registers to load them ahead: 85 us for 8-of-64 at 16 tokens, of which the
+// loads took 14).
+template <int NT, int STEP, int UPPER, int NTM, class Row, class Put>
+RLA_DEVFN bool moe_run_tiles(float (&acc)[2][NTM][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
                              volatile int* abort_flag, const Row& row, const Put& put) {
+  const int q = lane & 3;
   const __half* xp[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int col = t * 8 + (lane >> 2);
-    xp[t] = row(col < count ? col : 0) + k0 + (lane & 3) * 16;
+    xp[t] = row(col < count ? col : 0) + k0 + q * 16;
   }
+  int bytes = width - k0;  // from this stage's k on
+  MoeActs<NT> x;
+  if (NT == 1) x.load_first(xp, bytes, q);
+#pragma unroll 1
   for (int i = 0; i < n; ++i) {
-    const int bytes = width - k0 - i * moe::KB;
-    if (!(bytes >= moe::KB ? moe_stage<NT, true>(acc, ring, xp, bytes, lane, abort_flag)
-                           : moe_stage<NT, false>(acc, ring, xp, bytes, lane, abort_flag)))
-      return false;
+    MoeActs<NT> ahead;
+    if constexpr (NT == 1) {
+      const __half* next[1] = {xp[0] + moe::KB};
+      if (i + 1 < n) ahead.load_first(next, bytes - moe::KB, q);
+    } else {
+      x.load_first(xp, bytes, q);
+    }
+    uint32_t w;
+    if (!ring.wait(abort_flag, w)) return false;
+    moe_stage<NT, STEP, UPPER>(acc, w, x, xp, bytes, lane);
     __syncwarp();
     put();
 #pragma unroll
     for (int t = 0; t < NT; ++t) xp[t] += moe::KB;
+    bytes -= moe::KB;
+    if (NT == 1) x = ahead;
   }
   return true;
 }
-template <class Row, class Put>
-RLA_DEVFN bool moe_run(float (&acc)[4][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
+template <int STEP, int UPPER, int NTM, class Row, class Put>
+RLA_DEVFN bool moe_run(float (&acc)[2][NTM][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
                        volatile int* abort_flag, const Row& row, const Put& put) {
-  if (count <= 8) return moe_run_tiles<1>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
-  if (count <= 16) return moe_run_tiles<2>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
-  return moe_run_tiles<4>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+  if constexpr (NTM == 4)
+    if (count > 16) return moe_run_tiles<4, STEP, UPPER>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+  if constexpr (NTM >= 2)
+    if (count > 8) return moe_run_tiles<2, STEP, UPPER>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+  return moe_run_tiles<1, STEP, UPPER>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
 }
-RLA_DEVFN void moe_zero(float (&acc)[4][4]) {
+template <int NTM>
+RLA_DEVFN void moe_zero(float (&acc)[2][NTM][4]) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < NTM; ++t) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.f;
 }
 
 // Logits of this CTA's K slice, v[t][e] in 64 bits.  A warp takes 16 experts
@@ -352,16 +385,16 @@ RLA_DEVFN void moe_zero(float (&acc)[4][4]) {
 // 8-token tile's tokens.
 template <int NT>
 RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part, double* v) {
+  constexpr int WARPS = moe::warps(NT);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gr = lane >> 2, q = lane & 3;
-  const int etiles = (g.E + 15) / 16;  // at most WARPS
-  const int parts = moe::WARPS / etiles;
+  const int etiles = (g.E + 15) / 16;
+  const int parts = max(1, WARPS / etiles);
   const int blocks = (g.H + 31) / 32;  // 32 halves = one 8-half load of each of 4 lanes
-  if (warp < etiles * parts) {
-    const int e0 = warp % etiles * 16, sub = warp / etiles;
+  for (int item = warp; item < etiles * parts; item += WARPS) {
+    const int e0 = item % etiles * 16, sub = item / etiles;
     const int slices = moe::CLUSTER * parts, slice = rank * parts + sub;
-    const int b0 = static_cast<int>((int64_t)blocks * slice / slices);
-    const int b1 = static_cast<int>((int64_t)blocks * (slice + 1) / slices);
+    const int b0 = moe_part(blocks, slice, slices), b1 = moe_part(blocks, slice + 1, slices);
     const int r0 = min(e0 + gr, g.E - 1), r1 = min(e0 + gr + 8, g.E - 1);
     const __half* w0 = g.router + (int64_t)r0 * g.H + q * 8;
     const __half* w1 = g.router + (int64_t)r1 * g.H + q * 8;
@@ -389,7 +422,7 @@ RLA_DEVFN void moe_logits(const MoeArgs& g, int rank, float* part, double* v) {
       }
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < g.T * g.E; p += moe::THREADS) {
+  for (int p = threadIdx.x; p < g.T * g.E; p += 32 * WARPS) {
     double sum = 0;
 #pragma unroll 4
     for (int j = 0; j < parts; ++j) sum += static_cast<double>(part[j * g.T * g.E + p]);
@@ -412,7 +445,7 @@ RLA_DEVFN double moe_logit(long long key) {
 template <int PER>  // experts of a lane, at least E / 32
 RLA_DEVFN void moe_choose_of(const MoeArgs& g, const double* mine, MoeRoute& r) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int t = warp; t < g.T; t += moe::WARPS) {
+  for (int t = warp; t < g.T; t += blockDim.x >> 5) {
     double part[PER][moe::CLUSTER];
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -449,20 +482,22 @@ RLA_DEVFN void moe_choose_of(const MoeArgs& g, const double* mine, MoeRoute& r) 
       if (j == 0) top = moe_logit(k);
       if (lane == j) my_id = static_cast<int>(e), my_key = k;
     }
-    // softmax relative to the largest; a NaN logit makes the sum NaN
+    // softmax relative to the largest; a NaN logit makes the sum NaN.  (The
+    // intrinsics are a few ulp off; code that runs once is fetched from a busy
+    // L2, so it is kept short.)
     float total = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (left >> i & 1) total += expf(static_cast<float>(moe_logit(key[i]) - top));
+      if (left >> i & 1) total += __expf(static_cast<float>(moe_logit(key[i]) - top));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const float p = lane < g.top_k ? expf(static_cast<float>(moe_logit(my_key) - top)) / total : 0.f;
+    const float p = lane < g.top_k ? __fdividef(__expf(static_cast<float>(moe_logit(my_key) - top)), total) : 0.f;
     float chosen = p;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
     if (lane < g.top_k) {
       r.ids[t * g.top_k + lane] = my_id;
-      r.coef[t * g.top_k + lane] = g.renorm ? p / chosen : p;
+      r.coef[t * g.top_k + lane] = g.renorm ? __fdividef(p, chosen) : p;
       atomicOr(&r.mask[my_id], 1u << t);
     }
   }
@@ -478,30 +513,48 @@ RLA_DEVFN void moe_choose(const MoeArgs& g, const double* mine, MoeRoute& r) {
     moe_choose_of<8>(g, mine, r);
 }
 
-// A unit of the gate/up kernel: 8 gate rows and the same 8 up rows of one expert.
-RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int group, const float (&acc)[4][4], float sg,
-                               float su, int lane) {
-  const int q = lane & 3;
-  const int i = group * 8 + moe_row(lane >> 2), first = r.begin[e], count = __popc(r.mask[e]);
+// A unit of the gate/up kernel: 16 gate rows and the same 16 up rows of one
+// expert; a lane holds gate and up of the rows moe_row(lane / 4) and 8 + that.
+struct MoeUnitScales {
+  float gate[2], up[2];
+  RLA_DEVFN void load(const MoeArgs& g, int e, int group, int lane) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+    for (int m = 0; m < 2; ++m) {
+      const int64_t channel = (int64_t)e * g.I + group * 16 + m * 8 + moe_row(lane >> 2);
+      gate[m] = moe_scale(g.s_gate, g.scale_f32, channel);
+      up[m] = moe_scale(g.s_up, g.scale_f32, channel);
+    }
+  }
+};
+template <int NTM>
+RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int group, const float (&acc)[2][NTM][4],
+                               const MoeUnitScales& sc, int lane) {
+  const int q = lane & 3;
+  const int first = r.begin[e], count = __popc(r.mask[e]);
+#pragma unroll
+  for (int t = 0; t < NTM; ++t) {
     if (t * 8 >= count) break;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int col = t * 8 + 2 * q + j;
       if (col < count) {
-        const float gate = acc[t][j] * sg, up = acc[t][2 + j] * su;
-        // the down product's tensor-core operand is fp16: one rounding
-        g.a[(int64_t)r.entry[first + col] * g.I + i] = __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
+        __half* to = g.a + (int64_t)r.entry[first + col] * g.I + group * 16 + moe_row(lane >> 2);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const float gate = acc[m][t][j] * sc.gate[m], up = acc[m][t][2 + j] * sc.up[m];
+          // the down product's tensor-core operand is fp16: one rounding
+          to[m * 8] = __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
+        }
       }
     }
   }
 }
 
 template <int NT>  // tiles of 8 tokens
-__global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THREADS, 1)
+__global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(32 * moe::warps(NT), 1)
     moe_gate_up_kernel(const __grid_constant__ CUtensorMap gate_map, const __grid_constant__ CUtensorMap up_map,
                        const MoeArgs g, int stages) {
+  constexpr int WARPS = moe::warps(NT);
   extern __shared__ uint8_t moe_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 1023) & ~uintptr_t(1023));
   MoeShared& sm = *reinterpret_cast<MoeShared*>(smem);
@@ -517,21 +570,22 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
     rla_tma_prefetch_desc(&gate_map);
     rla_tma_prefetch_desc(&up_map);
   }
+  static_assert(32 * WARPS >= moe::MAX_E, "one thread an expert");
   if (threadIdx.x < moe::MAX_E) r.mask[threadIdx.x] = 0;
   rla_fence_barrier_init();
   rla_griddep_launch_dependents();
   {  // this CTA's part of the router into L2 while the previous kernel finishes
     const int64_t lines = ((int64_t)g.E * g.H * 2 + 127) / 128;
     const char* p = reinterpret_cast<const char*>(g.router);
-    for (int64_t i = rank * moe::THREADS + threadIdx.x; i < lines; i += moe::CLUSTER * moe::THREADS)
+    for (int64_t i = rank * 32 * WARPS + threadIdx.x; i < lines; i += moe::CLUSTER * 32 * WARPS)
       rla_prefetch_l2(p + i * 128);
   }
   rla_griddep_wait();
 
   // routing; its scratch lies in the ring, which is not in use yet
-  constexpr int PART = moe::WARPS * 16 * 8 * NT * 4;  // [parts][T][E] floats at most
+  constexpr int PART = 16 * 16 * 8 * NT * 4;  // [parts][T][E] floats at most (parts * E <= 256)
   constexpr int LOGITS = 8 * NT * moe::MAX_E * 8;
-  static_assert(PART + LOGITS <= moe::WARPS * 2 * moe::SLOT, "routing scratch fits the ring");
+  static_assert(PART + LOGITS <= WARPS * 2 * moe::SLOT, "routing scratch fits the ring");
   float* part = reinterpret_cast<float*>(rings);
   double* logits = reinterpret_cast<double*>(rings + PART);
   moe_logits<NT>(g, rank, part, logits);
@@ -543,25 +597,25 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   rla_fence_proxy_async();  // plain accesses to the ring come before the copies into it
 
   // This CTA's units, and of their stages this warp's run.
-  const int groups = g.I / 8;
+  const int groups = g.I / 16;
   const int per = (g.H + moe::KB - 1) / moe::KB;  // stages of a unit
   const int units = r.num_active * groups;
   const int u0 = moe_part(units, blockIdx.x, gridDim.x);
   const int items = (moe_part(units, blockIdx.x + 1, gridDim.x) - u0) * per;
-  const int i0 = moe_part(items, warp, moe::WARPS);
-  int left = moe_part(items, warp + 1, moe::WARPS) - i0;
+  const int i0 = moe_part(items, warp, WARPS);
+  int left = moe_part(items, warp + 1, WARPS) - i0;
   const int unit = u0 + i0 / per;
   int ca = unit / groups, cg = unit % groups, cs = i0 % per;  // the products' place
 
   int pa = ca, pg = cg, ps = cs, to_put = left;  // the copies' place
-  int prow = to_put > 0 ? r.active[pa] * g.I + pg * 8 : 0;
+  int prow = to_put > 0 ? r.active[pa] * g.I + pg * 16 : 0;
   auto put = [&]() {
     if (to_put == 0) return;
     --to_put;
-    ring.issue<2>(&gate_map, &up_map, ps * moe::KB, prow, g.H, lane);
+    ring.issue<2>(&gate_map, &up_map, ps * moe::KB, prow, lane);
     if (++ps == per) {
       ps = 0;
-      prow += 8;
+      prow += 16;
       if (++pg == groups) {
         pg = 0, ++pa;
         if (to_put > 0) prow = r.active[pa] * g.I;
@@ -572,68 +626,80 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(moe::THRE
   if (blockIdx.x == 0) {  // for the second kernel
     const uint4* from = reinterpret_cast<const uint4*>(static_cast<MoeTables*>(&r));
     uint4* to = reinterpret_cast<uint4*>(g.tables);
-    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 16); i += moe::THREADS) to[i] = from[i];
+    for (int i = threadIdx.x; i < (int)(sizeof(MoeTables) / 16); i += 32 * WARPS) to[i] = from[i];
   }
 
   bool head = left > 0 && cs != 0;  // the current unit began in an earlier warp
   bool tail = false, ok = true;
-  float acc[4][4], sg = 0.f, su = 0.f;
+  MoeAcc<NT> acc;
+  MoeUnitScales scales;
   moe_zero(acc);
-  while (left > 0) {
-    const int e = r.active[ca], first = r.begin[e];
-    const int n = min(per - cs, left);
-    // (read before the products, used after them)
-    const int64_t channel = (int64_t)e * g.I + cg * 8 + moe_row(lane >> 2);
-    sg = moe_scale(g.s_gate, g.scale_f32, channel);
-    su = moe_scale(g.s_up, g.scale_f32, channel);
-    ok = moe_run(acc, ring, n, cs * moe::KB, g.H, __popc(r.mask[e]), lane, &r.abort_flag,
-                 [&](int i) { return g.x + r.token[first + i] * g.ldx; }, put);
-    if (!ok) break;
-    left -= n;
-    cs += n;
-    if (head) {
-      float* h = heads + warp * NT * 128 + lane;
+  // One place finishes all units: code that a warp meets for the first time is
+  // fetched from an L2 that is busy with weights.
+  for (bool last = false; !last;) {
+    bool whole = false;
+    if (left > 0) {
+      const int e = r.active[ca], first = r.begin[e];
+      const int n = min(per - cs, left);
+      scales.load(g, e, cg, lane);  // (read before the products, used after them)
+      ok = moe_run<1024, moe::SLOT / 2>(acc, ring, n, cs * moe::KB, g.H, __popc(r.mask[e]), lane, &r.abort_flag,
+                                        [&](int i) { return g.x + r.token[first + i] * g.ldx; }, put);
+      left = ok ? left - n : 0;
+      cs += n;
+      if (!ok) {
+        ring.drain();
+      } else if (head) {
+        float* h = heads + warp * NT * 256 + lane;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[(t * 4 + j) * 32] = acc[t][j];
-      head = false;
-    } else if (cs == per) {
-      moe_finish_unit(g, r, e, cg, acc, sg, su, lane);
-    } else {
-      tail = true;  // goes on in the next warps; acc stays
-      break;
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[((m * NT + t) * 4 + j) * 32] = acc[m][t][j];
+        head = false;
+      } else {
+        whole = cs == per;
+        tail = !whole;  // goes on in the next warps
+      }
     }
+    last = left == 0;
+    if (last) {
+      __syncthreads();  // all heads are there
+      if (tail) {
+        const int end = (ca * groups + cg - u0 + 1) * per;  // the unit's last stage + 1
+        for (int w = warp + 1; w < WARPS; ++w) {
+          const int w0 = moe_part(items, w, WARPS), w1 = moe_part(items, w + 1, WARPS);
+          if (w0 >= end) break;
+          if (w0 == w1) continue;
+          const float* h = heads + w * NT * 256 + lane;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[m][t][j] += h[((m * NT + t) * 4 + j) * 32];
+        }
+        whole = true;
+      }
+    }
+    if (whole) moe_finish_unit(g, r, r.active[ca], cg, acc, scales, lane);
     if (cs == per) {
       cs = 0;
       if (++cg == groups) cg = 0, ++ca;
     }
     moe_zero(acc);
   }
-  if (!ok) ring.drain();
-  __syncthreads();
-  if (tail && ok) {
-    const int end = (ca * groups + cg - u0 + 1) * per;  // the unit's last stage + 1
-    for (int w = warp + 1; w < moe::WARPS; ++w) {
-      const int w0 = moe_part(items, w, moe::WARPS), w1 = moe_part(items, w + 1, moe::WARPS);
-      if (w0 >= end) break;
-      if (w0 == w1) continue;
-      const float* h = heads + w * NT * 128 + lane;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t][j] += h[(t * 4 + j) * 32];
-    }
-    moe_finish_unit(g, r, r.active[ca], cg, acc, sg, su, lane);
-  }
 }
 
-// Blocks of 16 output rows; of a block's (active expert, stage) list each
+// Blocks of 32 output rows; of a block's (active expert, stage) list each
 // warp of each of the `splits` CTAs of the cluster takes an equal run, and
 // adds each expert's part (x channel scale x token coefficient) to its sums
-// [T][16] in shared memory.
-__global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_constant__ CUtensorMap down_map,
-                                                                   const MoeArgs g, int stages) {
+// [T][32] in shared memory.  (Rows behind H in the last block belong to the
+// next expert, or are zeros; their sums are not stored.)
+template <int NT>  // tiles of 8 tokens
+__global__ void __launch_bounds__(32 * moe::warps(NT), 1)
+    moe_down_kernel(const __grid_constant__ CUtensorMap down_map, const MoeArgs g, int stages) {
+  constexpr int WARPS = moe::warps(NT);
   extern __shared__ uint8_t moe_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(moe_smem) + 1023) & ~uintptr_t(1023));
   MoeShared& sm = *reinterpret_cast<MoeShared*>(smem);
@@ -655,15 +721,15 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_
     const uint4* from = reinterpret_cast<const uint4*>(g.tables);
     uint4* to = reinterpret_cast<uint4*>(static_cast<MoeTables*>(&r));
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(MoeTables) / 16); i += moe::THREADS)
+    for (int i = 0; i < (int)(sizeof(MoeTables) / 16); i += 32 * WARPS)
       if (i + threadIdx.x < sizeof(MoeTables) / 16) to[i + threadIdx.x] = __ldcg(from + i + threadIdx.x);
   }
   __syncthreads();
 
-  const int blocks = g.H / 16;
+  const int blocks = (g.H + moe::ROWS - 1) / moe::ROWS;
   const int per = (g.I + moe::KB - 1) / moe::KB;
   const int items = r.num_active * per;
-  const int parts = splits * moe::WARPS, mine = split * moe::WARPS + warp;
+  const int parts = splits * WARPS, mine = split * WARPS + warp;
   const int i0 = moe_part(items, mine, parts), n = moe_part(items, mine + 1, parts) - i0;
   const int a0 = i0 / per, s0 = i0 - a0 * per;
 
@@ -671,14 +737,14 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_
   int pb = blockIdx.x, pa = a0, ps = s0, pi = 0;
   auto put = [&]() {
     if (n == 0 || pb >= blocks) return;
-    ring.issue<1>(&down_map, nullptr, ps * moe::KB, r.active[pa] * g.H + pb * 16, g.I, lane);
+    ring.issue<1>(&down_map, nullptr, ps * moe::KB, r.active[pa] * g.H + pb * moe::ROWS, lane);
     if (++ps == per) ps = 0, ++pa;
     if (++pi == n) pi = 0, pa = a0, ps = s0, pb += gridDim.x;
   };
   for (int i = 0; i < stages; ++i) put();
 
   bool ok = true;
-  const int values = g.T * 16;
+  const int values = g.T * moe::ROWS;
   float* own = sums + warp * values;
   for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
     for (int p = lane; p < values; p += 32) own[p] = 0.f;
@@ -686,26 +752,29 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_
     while (left > 0 && ok) {
       const int e = r.active[ca], first = r.begin[e], count = __popc(r.mask[e]);
       const int m = min(per - cs, left);
-      // (read before the products, used after them)
-      const float sa = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr);
-      const float sb = moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + b * 16 + gr + 8);
-      float acc[4][4];
+      float scale[2][2];  // (read before the products, used after them)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        scale[i >> 1][i & 1] =
+            moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + min(b * moe::ROWS + gr + i * 8, g.H - 1));
+      MoeAcc<NT> acc;
       moe_zero(acc);
-      ok = moe_run(acc, ring, m, cs * moe::KB, g.I, count, lane, &r.abort_flag,
-                   [&](int i) { return g.a + (int64_t)r.entry[first + i] * g.I; }, put);
+      ok = moe_run<2048, 1024>(acc, ring, m, cs * moe::KB, g.I, count, lane, &r.abort_flag,
+                               [&](int i) { return g.a + (int64_t)r.entry[first + i] * g.I; }, put);
       if (!ok) break;
       __syncwarp();  // the zeros, or another expert's sums, are in place
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < NT; ++t) {
         if (t * 8 >= count) break;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int col = t * 8 + 2 * q + j;
           if (col < count) {
             const float c = r.coef[r.entry[first + col]];
-            float* v = own + r.token[first + col] * 16 + gr;
-            v[0] = fmaf(acc[t][j] * sa, c, v[0]);
-            v[8] = fmaf(acc[t][2 + j] * sb, c, v[8]);
+            float* v = own + r.token[first + col] * moe::ROWS + gr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i * 8] = fmaf(acc[i >> 1][t][2 * (i & 1) + j] * scale[i >> 1][i & 1], c, v[i * 8]);
           }
         }
       }
@@ -714,18 +783,19 @@ __global__ void __launch_bounds__(moe::THREADS, 1) moe_down_kernel(const __grid_
     }
     __syncthreads();
     // the CTA's sum into warp 0's (each thread its own values), then the ranks'
-    for (int p = threadIdx.x; p < values; p += moe::THREADS) {
+    for (int p = threadIdx.x; p < values; p += 32 * WARPS) {
       float v = sums[p];
 #pragma unroll
-      for (int w = 1; w < moe::WARPS; ++w) v += sums[w * values + p];
+      for (int w = 1; w < WARPS; ++w) v += sums[w * values + p];
       sums[p] = v;
     }
     if (splits > 1) rla_cluster_sync();
     if (split == 0) {
-      for (int p = threadIdx.x; p < values; p += moe::THREADS) {
+      for (int p = threadIdx.x; p < values; p += 32 * WARPS) {
         float v = sums[p];
         for (int c = 1; c < splits; ++c) v += rla_ld_dsmem_f32(&sums[p], c);
-        g.y[(int64_t)(p / 16) * g.ldy + b * 16 + p % 16] = __float2half_rn(v);
+        const int row = b * moe::ROWS + p % moe::ROWS;
+        if (row < g.H) g.y[(int64_t)(p / moe::ROWS) * g.ldy + row] = __float2half_rn(v);
       }
     }
     if (splits > 1)
@@ -751,7 +821,7 @@ static int moe_up_clusters(size_t smem) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(moe::CLUSTER);
-  cfg.blockDim = dim3(moe::THREADS);
+  cfg.blockDim = dim3(32 * moe::warps(NT));
   cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -773,36 +843,36 @@ template <int NT>
 static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   CUtensorMap gate_map, up_map, down_map;
   const uint64_t E = g.E, H = g.H, I = g.I;
-  if (!make_tmap_2d(&gate_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_gate, H, E * I, H, 128, 8, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_2d(&up_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_up, H, E * I, H, 128, 8, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_2d(&down_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_down, I, E * H, I, 128, 16, CU_TENSOR_MAP_SWIZZLE_128B))
+  if (!make_tmap_2d(&gate_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_gate, H, E * I, H, 128, 16, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&up_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_up, H, E * I, H, 128, 16, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&down_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.w_down, I, E * H, I, 128, 32, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   const int sms = device_sm_count();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(moe::THREADS);
+  cfg.blockDim = dim3(32 * moe::warps(NT));
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
 
-  int stages = moe::MAX_STAGES;  // 3 up to 16 tokens, 2 above
+  int stages = moe::MAX_STAGES;  // 3 up to 8 tokens and above 16, 2 between
   while (moe_smem_bytes(g.T, stages) > moe::SMEM) --stages;
   cfg.dynamicSmemBytes = moe_smem_bytes(g.T, stages);
   cudaError_t e = cudaFuncSetAttribute(moe_gate_up_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)cfg.dynamicSmemBytes);
   if (e != cudaSuccess) return e;
-  const int64_t most = (int64_t)std::min(g.E, g.T * g.top_k) * (g.I / 8);  // units, at most
+  const int64_t most = (int64_t)std::min(g.E, g.T * g.top_k) * (g.I / 16);  // units, at most
   const int64_t clusters = std::min<int64_t>(moe_up_clusters<NT>(cfg.dynamicSmemBytes),
                                              (most + moe::CLUSTER - 1) / moe::CLUSTER);
   cfg.gridDim = dim3((unsigned)(clusters * moe::CLUSTER));
   e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, gate_map, up_map, g, stages);
   if (e != cudaSuccess) return e;
 
-  e = cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+  e = cudaFuncSetAttribute(moe_down_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
   if (e != cudaSuccess) return e;
-  const int blocks = g.H / 16;
+  const int blocks = (g.H + moe::ROWS - 1) / moe::ROWS;
   const int splits = std::max(1, std::min(moe::MAX_SPLITS, sms / blocks));
   cfg.gridDim = dim3(splits > 1 ? blocks : std::min(blocks, sms), splits);
   if (splits > 1) {
@@ -812,7 +882,7 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, moe_down_kernel, down_map, g, stages);
+  return cudaLaunchKernelEx(&cfg, moe_down_kernel<NT>, down_map, g, stages);
 }
 
 static int moe_fail(int code, const char* msg) {
