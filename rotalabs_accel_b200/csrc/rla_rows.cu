@@ -400,7 +400,7 @@ static cudaError_t launch_rows_stream_cfg(const RowsArgs& g, int op, cudaStream_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   auto run = [&](auto kern) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, budget);
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kern, g, stages, row_bytes);
   };
   switch (op) {

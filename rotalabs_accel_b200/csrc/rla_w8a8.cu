@@ -7,7 +7,7 @@
 // tile, the split of K or the number of CTAs.
 //
 // Orientation: a tile is 128 (or, of a CTA pair, 256) output channels (the
-// MMA's M, the TMEM lanes) x up to 256 tokens (the MMA's N), so the channel's
+// MMA's M, the TMEM lanes) x up to 128 (256) tokens (the MMA's N), so the channel's
 // scale and bias are two registers of an epilogue thread, and one token costs
 // 16 columns, not 128 rows.
 //
@@ -28,6 +28,7 @@
 // blocks, 128-byte swizzle), warp 1 TMEM allocation and MMA issue, warps 2-5
 // epilogue (one TMEM lane quarter each).  All waits are bounded.
 #include <algorithm>
+#include <atomic>
 
 #include "rla_common.cuh"
 #include "rla_internal.h"
@@ -39,7 +40,8 @@ namespace w8 {
 constexpr int BR = 128;       // output channels of a tile
 constexpr int BK = 128;       // k (bytes) of a stage: one 128-byte swizzle row
 constexpr int THREADS = 192;
-constexpr int MAX_STAGES = 12;
+constexpr int MAX_STAGES = 4;
+constexpr int MAX_BT = 128;    // token columns of a split tile
 constexpr int MAX_SPLITS = 8;  // portable cluster size
 constexpr int MAX_K = 131071;  // K * 128 * 128 < 2^31
 __host__ __device__ constexpr int stage_bytes(int bt) { return (BR + bt) * BK; }
@@ -170,7 +172,7 @@ RLA_DEVFN __half w8a8_value(int sum, float sw, float sx, float bias) {
   return __float2half_rn(fmaf(static_cast<float>(sum) * sw, sx, bias));
 }
 
-// bt: token columns of a tile, a multiple of 16 up to 256.
+// bt: token columns of a tile, a multiple of 16 up to MAX_BT.
 __global__ void __launch_bounds__(w8::THREADS)
     w8a8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                       const W8Out out, int num_kb, int stages, int bt, int tmem_cols) {
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(w8::THREADS)
   __shared__ uint64_t full[w8::MAX_STAGES], empty[w8::MAX_STAGES], dfull;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_word;
-  __shared__ float sx_s[256];
+  __shared__ float sx_s[w8::MAX_BT];
   __shared__ __align__(16) float sw_s[w8::BR], bias_s[w8::BR];
 
   const int warp = threadIdx.x >> 5;
@@ -525,46 +527,104 @@ __global__ void w8a8_align_rows_kernel(const int8_t* __restrict__ src, int64_t l
 
 struct W8Plan {
   bool pair = false;
-  int bt = 0, splits = 1, per_sm = 1, stages = 0;
+  int bt = 0, splits = 1, stages = 0;
   int grid_x = 0, grid_y = 0;
   size_t smem = 0;
 };
 
-// K slices and CTAs per SM: the pair with the shortest estimated time, in k
-// blocks of one SM's share of the memory system -- rounds of resident CTAs x
-// the k blocks a CTA streams, plus a fixed cost a round.
+// Dynamic shared memory of the split kernel, at most (its attribute is set to
+// this, whatever a launch takes: calls on several host threads may interleave).
+constexpr int kW8SplitSmem = w8::MAX_STAGES * w8::stage_bytes(w8::MAX_BT) + 1024;
+
+// CTAs that run at once, one an SM, when `splits` of them form a cluster (whole
+// clusters: all CTAs of one sit in one GPC).  Per device.
+static int w8a8_cluster_ctas(int splits) {
+  static std::atomic<int> cache[64][w8::MAX_SPLITS + 1];
+  const int sms = device_sm_count();
+  int dev = -1;
+  if (splits == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms / splits * splits;
+  int n = cache[dev][splits].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  cudaError_t e = cudaFuncSetAttribute(w8a8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW8SplitSmem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1, 1, splits);
+  cfg.blockDim = dim3(w8::THREADS);
+  cfg.dynamicSmemBytes = kW8SplitSmem;  // more than half an SM's
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = static_cast<unsigned>(splits);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, w8a8_split_kernel, &cfg);
+  if (e != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    return sms / splits * splits;  // (no device: planning only)
+  }
+  cache[dev][splits].store(n * splits, std::memory_order_relaxed);
+  return n * splits;
+}
+// Split CTAs that an SM holds with this ring: the dynamic shared memory, the
+// static and the system's.  (The occupancy query counts one an SM for a kernel
+// that allocates Tensor Memory; as many run as fit.)
+static int w8a8_per_sm(int bt, int stages) { return 228 * 1024 / (stages * w8::stage_bytes(bt) + 4 * 1024); }
+
+// Which kernel, tile, split of K and ring, by estimated time.  Measured on
+// B200 (CUDA graphs, inputs beyond L2), over token tiles of 64 to 256, 1 to 8
+// slices and rings of 2 to 12 stages:
+//  - Several CTAs an SM with short rings, whose starts and ends overlap one
+//    another's streams (and the next launch's start), beat one CTA with the
+//    whole shared memory: 8x28672x8192 38 us against 83, 16x14336x4096 13.5
+//    against 16.6, 1x4096x4096 6.4 against 7.9.  So token tiles of at most
+//    128 columns and two or three stages.
+//  - A round of n CTAs an SM takes about 0.31 + 0.16 n us a k block (256x4096,
+//    512x4096, 512x11008, K = 4096), a seventh more with two stages.
+//  - Joining the slices takes about 2.4 us for a tile of 128 tokens, in
+//    proportion for narrower ones, and longer where several CTAs of an SM do
+//    it: 3000x512x512 8.9 us unsplit, 13.7 as two slices.
+//  - A round starts and ends in about 1.5 us: 1x28672x1024 8.3 us as 3 slices
+//    in one round, 16.4 as 8 in three.
+//  - Slices whose clusters do not all fit at once cost a second round
+//    (300x4096x4096: 21.8 us as 3, 16.1 as 2).
+//  - A round of CTA pairs (256 x 256 tiles) takes about 0.5 us a k block:
+//    2048x4096x4096 pairs 35.2 us, split 43.8; 512x11008x4096 35.3 and 29.9.
 static W8Plan w8a8_plan(int64_t M, int64_t N, int64_t K) {
   W8Plan p;
   const int sms = device_sm_count();
   const int kb = static_cast<int>((K + w8::BK - 1) / w8::BK);
-  const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256);
-  if (M > 128 && 2 * pair_tiles >= sms) {
-    p.pair = true;
-    return p;
-  }
-  // Token tiles of equal width, a multiple of 16 columns, at most 256.
-  p.grid_y = static_cast<int>((M + 255) / 256);
+  // token tiles of equal width, a multiple of 16 columns
+  p.grid_y = static_cast<int>((M + 127) / 128);
   p.bt = static_cast<int>(((M + p.grid_y - 1) / p.grid_y + 15) / 16 * 16);
   p.grid_x = static_cast<int>((N + w8::BR - 1) / w8::BR);
   const int64_t tiles = (int64_t)p.grid_x * p.grid_y;
   const int stage = w8::stage_bytes(p.bt);
-  double best = 0;
-  for (int c = 1; c <= (p.bt <= 32 ? 4 : p.bt <= 64 ? 2 : 1); ++c) {
-    const int ring = (c == 1 ? 220 : c == 2 ? 108 : c == 3 ? 70 : 52) * 1024;
-    int stages = ring / stage;
-    if (stages > w8::MAX_STAGES) stages = w8::MAX_STAGES;
-    for (int s = 1; s <= w8::MAX_SPLITS && s <= kb; ++s) {
-      const int64_t rounds = (tiles * s + (int64_t)sms * c - 1) / ((int64_t)sms * c);
-      const double cost = static_cast<double>(rounds) * c * ((kb + s - 1) / s + 1) + (s > 1 ? 1.0 : 0.0);
-      if (best == 0 || cost < best) {
-        best = cost;
+  double best = -1;
+  for (int s = 1; s <= w8::MAX_SPLITS && s <= kb; ++s) {
+    for (int st = 3; st >= 2; --st) {
+      if (s > 1 && st * stage < p.bt * w8::BR * 4) continue;  // no room for the partial tile
+      const int c = w8a8_per_sm(p.bt, st);
+      const int64_t slots = (int64_t)c * w8a8_cluster_ctas(s), rounds = (tiles * s + slots - 1) / slots;
+      const int64_t n = rounds > 1 ? c : std::min<int64_t>(c, (tiles * s + sms - 1) / sms);
+      double us = static_cast<double>(rounds) * ((kb + s - 1) / s) * (0.31 + 0.16 * n) * (st == 2 ? 1.15 : 1.0);
+      us += 1.5 * rounds;
+      if (s > 1) us += 2.4 * p.bt / 128 * (1 + 0.5 * (n - 1));
+      if (best < 0 || us < best) {
+        best = us;
         p.splits = s;
-        p.per_sm = c;
-        p.stages = stages;
+        p.stages = st;
       }
     }
   }
+  if (tiles * p.splits <= w8a8_cluster_ctas(p.splits)) p.stages = w8::MAX_STAGES;  // one CTA an SM: room for more
+  // (no more stages than k blocks, but room for the partial tile)
+  p.stages = std::max(std::min(p.stages, (kb + p.splits - 1) / p.splits),
+                      p.splits > 1 ? (p.bt * w8::BR * 4 + stage - 1) / stage : 1);
   p.smem = (size_t)p.stages * stage + 1024;
+  if (M > 128) {
+    const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256), pairs = std::max(1, sms / 2);
+    p.pair = static_cast<double>((pair_tiles + pairs - 1) / pairs) * kb * 0.5 + 1.5 < best;
+  }
   return p;
 }
 
@@ -602,7 +662,7 @@ static cudaError_t launch_w8a8(const int8_t* x, int64_t ldx, const int8_t* w, in
     if (e != cudaSuccess) return e;
     return cudaLaunchKernelEx(&cfg, w8a8_pair_kernel, tw, tx, out, num_kb, order);
   }
-  cudaError_t e = cudaFuncSetAttribute(w8a8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  cudaError_t e = cudaFuncSetAttribute(w8a8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW8SplitSmem);
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3(p.grid_x, p.grid_y, p.splits);
   cfg.dynamicSmemBytes = p.smem;
