@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/rla_w8a16.h"
 
 namespace rla {
@@ -87,6 +89,21 @@ constexpr int kMaxClusterSplits = 8;
 
 // peer: plan for the launch with the fused peer exchange (its own occupancy)
 Plan make_plan(int64_t M, int64_t N, int64_t K, bool aligned, bool have_workspace, bool peer = false);
+
+// Allows `kernel` up to `bytes` of dynamic shared memory, once per device
+// (`done`: a bit per device, of this kernel).  Always the kernel's maximum, not
+// a launch's need: launches on several host threads may interleave.
+template <class Kernel>
+inline cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (set == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return set;
+}
 
 void note_launch();
 int device_sm_count();  // SMs of the current device (148 if it cannot be read)

@@ -860,8 +860,8 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   int stages = moe::MAX_STAGES;  // 3 up to 8 tokens and above 16, 2 between
   while (moe_smem_bytes(g.T, stages) > moe::SMEM) --stages;
   cfg.dynamicSmemBytes = moe_smem_bytes(g.T, stages);
-  cudaError_t e = cudaFuncSetAttribute(moe_gate_up_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)moe::SMEM);
+  static std::atomic<uint64_t> up_done{0}, down_done{0};
+  cudaError_t e = allow_smem(moe_gate_up_kernel<NT>, (int)moe::SMEM, up_done);
   if (e != cudaSuccess) return e;
   const int64_t most = (int64_t)std::min(g.E, g.T * g.top_k) * (g.I / 16);  // units, at most
   const int64_t clusters = std::min<int64_t>(moe_up_clusters<NT>(cfg.dynamicSmemBytes),
@@ -870,7 +870,7 @@ static cudaError_t launch_moe(const MoeArgs& g, cudaStream_t s) {
   e = cudaLaunchKernelEx(&cfg, moe_gate_up_kernel<NT>, gate_map, up_map, g, stages);
   if (e != cudaSuccess) return e;
 
-  e = cudaFuncSetAttribute(moe_down_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)moe::SMEM);
+  e = allow_smem(moe_down_kernel<NT>, (int)moe::SMEM, down_done);
   if (e != cudaSuccess) return e;
   const int blocks = (g.H + moe::ROWS - 1) / moe::ROWS;
   const int splits = std::max(1, std::min(moe::MAX_SPLITS, sms / blocks));

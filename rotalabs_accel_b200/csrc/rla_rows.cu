@@ -399,8 +399,9 @@ static cudaError_t launch_rows_stream_cfg(const RowsArgs& g, int op, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  static std::atomic<uint64_t> done[3];
   auto run = [&](auto kern) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, budget);
+    const cudaError_t e = allow_smem(kern, budget, done[op]);
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kern, g, stages, row_bytes);
   };
   switch (op) {

@@ -532,9 +532,12 @@ struct W8Plan {
   size_t smem = 0;
 };
 
-// Dynamic shared memory of the split kernel, at most (its attribute is set to
-// this, whatever a launch takes: calls on several host threads may interleave).
+// Dynamic shared memory of the split kernel, at most.
 constexpr int kW8SplitSmem = w8::MAX_STAGES * w8::stage_bytes(w8::MAX_BT) + 1024;
+static cudaError_t w8a8_allow_split_smem() {
+  static std::atomic<uint64_t> done{0};
+  return allow_smem(w8a8_split_kernel, kW8SplitSmem, done);
+}
 
 // CTAs that run at once, one an SM, when `splits` of them form a cluster (whole
 // clusters: all CTAs of one sit in one GPC).  Per device.
@@ -545,7 +548,7 @@ static int w8a8_cluster_ctas(int splits) {
   if (splits == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms / splits * splits;
   int n = cache[dev][splits].load(std::memory_order_relaxed);
   if (n > 0) return n;
-  cudaError_t e = cudaFuncSetAttribute(w8a8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW8SplitSmem);
+  cudaError_t e = w8a8_allow_split_smem();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1, 1, splits);
   cfg.blockDim = dim3(w8::THREADS);
@@ -657,12 +660,12 @@ static cudaError_t launch_w8a8(const int8_t* x, int64_t ldx, const int8_t* w, in
     const int pairs = static_cast<int>(std::min<int64_t>(tiles, device_sm_count() / 2));
     cfg.gridDim = dim3(2 * pairs);
     cfg.dynamicSmemBytes = sizeof(W8PairShared) + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(w8a8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)cfg.dynamicSmemBytes);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(w8a8_pair_kernel, (int)cfg.dynamicSmemBytes, done);
     if (e != cudaSuccess) return e;
     return cudaLaunchKernelEx(&cfg, w8a8_pair_kernel, tw, tx, out, num_kb, order);
   }
-  cudaError_t e = cudaFuncSetAttribute(w8a8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW8SplitSmem);
+  const cudaError_t e = w8a8_allow_split_smem();
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3(p.grid_x, p.grid_y, p.splits);
   cfg.dynamicSmemBytes = p.smem;

@@ -61,6 +61,23 @@ def int8_moe(x: torch.Tensor, router_weight: torch.Tensor, w_gate: torch.Tensor,
     Returns ``(..., H)``, fp16 for CUDA inputs, ``x.dtype`` for CPU inputs.
     On CUDA: E <= 256, top_k <= 32, H and I multiples of 16.
     """
+    if x.is_cuda and x.dim() == 2 and x.dtype == torch.float16:
+        # (the per-token case: the extension checks; see w8a8.py)
+        try:
+            return _capi.torch_ops().moe(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down,
+                                         top_k, renormalize)
+        except RuntimeError:
+            _moe_args(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k)
+            raise
+    _moe_args(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k)
+    if x.is_cuda:
+        y = _capi.torch_ops().moe(_as_2d_fp16(x, x.shape[-1]), router_weight, w_gate, scale_gate, w_up, scale_up,
+                                  w_down, scale_down, top_k, renormalize)
+        return y.view(x.shape)
+    return int8_moe_torch(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k, renormalize)
+
+
+def _moe_args(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k):
     assert w_gate.dtype == torch.int8 and w_up.dtype == torch.int8 and w_down.dtype == torch.int8, \
         "Weight must be INT8"
     E, H = router_weight.shape
@@ -72,12 +89,6 @@ def int8_moe(x: torch.Tensor, router_weight: torch.Tensor, w_gate: torch.Tensor,
         f"Scale shape mismatch: {tuple(scale_gate.shape)} / {tuple(scale_up.shape)} / {tuple(scale_down.shape)}"
     if not 1 <= top_k <= E:
         raise ValueError(f"top_k must be in [1, {E}], got {top_k}")
-    if x.is_cuda:
-        x2 = x if x.dim() == 2 and x.dtype == torch.float16 else _as_2d_fp16(x, H)
-        y = _capi.torch_ops().moe(x2, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k,
-                                  renormalize)
-        return y if x.dim() == 2 else y.view(x.shape)
-    return int8_moe_torch(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k, renormalize)
 
 
 class Int8MoE(torch.nn.Module):

@@ -62,6 +62,24 @@ def _norm_args(x, residual, weight):
         f"Residual shape mismatch: {tuple(residual.shape)} vs {tuple(x.shape)}"
 
 
+def _swiglu_args(gate, up):
+    assert gate.shape == up.shape, f"Gate and up shape mismatch: {tuple(gate.shape)} vs {tuple(up.shape)}"
+
+
+def _w8a8_args(x_int8, x_scale, weight_int8, scale):
+    assert x_int8.dtype == torch.int8, "Activations must be INT8"
+    assert weight_int8.dtype == torch.int8, "Weight must be INT8"
+    K, N = x_int8.shape[-1], weight_int8.shape[0]
+    assert weight_int8.shape == (N, K), f"Weight shape mismatch: {weight_int8.shape} vs ({N}, {K})"
+    assert x_scale.shape == x_int8.shape[:-1], \
+        f"Activation scale shape mismatch: {tuple(x_scale.shape)} vs {tuple(x_int8.shape[:-1])}"
+    assert scale.shape == (N,), f"Scale shape mismatch: {scale.shape} vs ({N},)"
+
+
+# 2-D CUDA operands, the per-token case, go straight to the extension, which
+# checks them; what it refuses is checked once more here, so that a mismatch of
+# shapes is the same AssertionError everywhere.
+
 def add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6):
     """``h = x + residual`` (rounded to ``x.dtype``; ``x`` itself where
     ``residual`` is None) and ``y = rmsnorm(h)``: returns ``(y, h)``, both of
@@ -69,10 +87,14 @@ def add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch
 
     x, residual: ``(..., K)`` fp16 or bf16 (the same); weight ``(K,)`` fp32,
     fp16 or bf16.  The norm is taken of the rounded sum, in fp32."""
+    if x.is_cuda and x.dim() == 2:
+        try:
+            return _capi.torch_ops().add_rmsnorm(x, residual, weight, eps)
+        except RuntimeError:
+            _norm_args(x, residual, weight)
+            raise
     _norm_args(x, residual, weight)
     if x.is_cuda:
-        if x.dim() == 2:
-            return _capi.torch_ops().add_rmsnorm(x, residual, weight, eps)
         y, h = _capi.torch_ops().add_rmsnorm(_rows(x), _rows(residual), weight, eps)
         return y.view(x.shape), x if residual is None else h.view(x.shape)
     v, h = _norm_torch(x, residual, weight, eps)
@@ -85,10 +107,14 @@ def add_rmsnorm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
     ``max|row| / 127``, 1 for a zero row) and ``h`` as in ``add_rmsnorm``.
     ``q * scale`` is what ``int8_gemm_w8a8`` multiplies.  A row holding an
     infinity or NaN gets the scale NaN and ``q = 0``."""
+    if x.is_cuda and x.dim() == 2:
+        try:
+            return _capi.torch_ops().add_rmsnorm_int8(x, residual, weight, eps)
+        except RuntimeError:
+            _norm_args(x, residual, weight)
+            raise
     _norm_args(x, residual, weight)
     if x.is_cuda:
-        if x.dim() == 2:
-            return _capi.torch_ops().add_rmsnorm_int8(x, residual, weight, eps)
         q, s, h = _capi.torch_ops().add_rmsnorm_int8(_rows(x), _rows(residual), weight, eps)
         return q.view(x.shape), s.view(x.shape[:-1]), x if residual is None else h.view(x.shape)
     v, h = _norm_torch(x, residual, weight, eps)
@@ -99,10 +125,14 @@ def add_rmsnorm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
 def swiglu_int8(gate: torch.Tensor, up: torch.Tensor):
     """``silu(gate) * up`` (fp32) in int8: returns ``(q, scale)`` as
     ``add_rmsnorm_int8`` does.  gate, up: ``(..., N)`` fp16 or bf16."""
-    assert gate.shape == up.shape, f"Gate and up shape mismatch: {tuple(gate.shape)} vs {tuple(up.shape)}"
-    if gate.is_cuda:
-        if gate.dim() == 2:
+    if gate.is_cuda and gate.dim() == 2:
+        try:
             return _capi.torch_ops().swiglu_int8(gate, up)
+        except RuntimeError:
+            _swiglu_args(gate, up)
+            raise
+    _swiglu_args(gate, up)
+    if gate.is_cuda:
         q, s = _capi.torch_ops().swiglu_int8(_rows(gate), _rows(up))
         return q.view(gate.shape), s.view(gate.shape[:-1])
     return _quantize_rows(torch.nn.functional.silu(gate.float()) * up.float())
@@ -117,19 +147,16 @@ def int8_gemm_w8a8(x_int8: torch.Tensor, x_scale: torch.Tensor, weight_int8: tor
     ``(N,)`` fp16 or fp32.  Returns fp16 ``(..., N)``.  The sum over K is
     exact (int32), so K < 131072; any strides, sizes and alignment (rows that
     are not 16-byte aligned are copied first)."""
-    assert x_int8.dtype == torch.int8, "Activations must be INT8"
-    assert weight_int8.dtype == torch.int8, "Weight must be INT8"
-    K = x_int8.shape[-1]
-    N = weight_int8.shape[0]
-    assert weight_int8.shape == (N, K), f"Weight shape mismatch: {weight_int8.shape} vs ({N}, {K})"
-    assert x_scale.shape == x_int8.shape[:-1], \
-        f"Activation scale shape mismatch: {tuple(x_scale.shape)} vs {tuple(x_int8.shape[:-1])}"
-    assert scale.shape == (N,), f"Scale shape mismatch: {scale.shape} vs ({N},)"
-    if x_int8.is_cuda:
-        if x_int8.dim() == 2:
+    if x_int8.is_cuda and x_int8.dim() == 2:
+        try:
             return _capi.torch_ops().w8a8_gemm(x_int8, x_scale, weight_int8, scale, bias)
+        except RuntimeError:
+            _w8a8_args(x_int8, x_scale, weight_int8, scale)
+            raise
+    _w8a8_args(x_int8, x_scale, weight_int8, scale)
+    if x_int8.is_cuda:
         y = _capi.torch_ops().w8a8_gemm(_rows(x_int8), x_scale.reshape(x_scale.numel()), weight_int8, scale, bias)
-        return y.view(*x_int8.shape[:-1], N)
+        return y.view(*x_int8.shape[:-1], weight_int8.shape[0])
     # products of int8 summed in fp64: exact, as on the GPU
     y = (x_int8.double() @ weight_int8.double().t()).float() * scale.float() * x_scale.unsqueeze(-1)
     return (y if bias is None else y + bias.float()).half()

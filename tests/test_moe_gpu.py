@@ -174,6 +174,12 @@ def test_types_strides_and_refusals(cuda_lib):
         ra.int8_moe(*p[:7], p[7].half(), top_k=2)
     with pytest.raises(RuntimeError, match="same CUDA device"):
         ra.int8_moe(x, p[1].cpu(), *p[2:], top_k=2)
+    with pytest.raises(AssertionError, match="Weight must be INT8"):
+        ra.int8_moe(*p[:2], p[2].float(), *p[3:], top_k=2)
+    with pytest.raises(AssertionError, match="Scale shape mismatch"):
+        ra.int8_moe(*p[:3], p[3][:, :5], *p[4:], top_k=2)
+    with pytest.raises(ValueError, match="top_k"):
+        ra.int8_moe(*p, top_k=13)
     odd = _problem(3, 72, 40, 4)
     with pytest.raises(RuntimeError, match="multiples of 16"):
         ra.int8_moe(*odd, top_k=2)

@@ -300,7 +300,18 @@ def test_gpu_refusals(cuda_lib):
         ra.add_rmsnorm(x.half(), x.half().cpu(), w)
     with pytest.raises(RuntimeError, match="eps"):
         ra.add_rmsnorm(x.half(), None, w, -1.0)
+    with pytest.raises(AssertionError, match="Hidden dim mismatch"):
+        ra.add_rmsnorm(x.half(), None, w[:5])
+    with pytest.raises(AssertionError, match="Residual shape mismatch"):
+        ra.add_rmsnorm_int8(x.half(), x.half()[:1], w)
+    with pytest.raises(AssertionError, match="Gate and up shape"):
+        ra.swiglu_int8(x.half(), x.half()[:, :5])
     q, s = torch.zeros(2, 64, dtype=torch.int8, device="cuda"), torch.ones(2, device="cuda")
+    for args, what in (((x, s, q, s), "Activations must be INT8"), ((q, s, x, s), "Weight must be INT8"),
+                       ((q, s, q[:, :5], s), "Weight shape mismatch"), ((q, s[:1], q, s), "Activation scale shape"),
+                       ((q, s, q, s[:1]), "Scale shape mismatch")):
+        with pytest.raises(AssertionError, match=what):
+            ra.int8_gemm_w8a8(*args)
     with pytest.raises(RuntimeError, match="same CUDA device"):
         ra.int8_gemm_w8a8(q, s, q.cpu(), s)
     with pytest.raises(TypeError, match="x_scale must be float32"):
