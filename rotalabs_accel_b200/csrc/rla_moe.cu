@@ -28,9 +28,9 @@
 //
 // Routing.  Which weights to read is not known before the logits are, so
 // the whole GPU waits for them.  Each cluster of 4 CTAs computes all logits by
-// itself (K split over its CTAs, joined through distributed shared memory),
-// and each CTA makes all choices for itself: no grid-wide barrier, one kernel
-// launch less, and 1/4 of the router's bytes an SM.  A choice between two experts is a border, so the partial logits
+// itself (K split over its CTAs, joined through distributed shared memory):
+// no grid-wide barrier, one kernel launch less, and 1/4 of the router's bytes
+// an SM.  A choice between two experts is a border, so the partial logits
 // (fp32 sums over 1/4 of K or less) are added in 64 bits.  Ties go to the
 // lower index.
 //
@@ -99,6 +99,14 @@ struct MoeArgs {
 
 RLA_DEVFN float moe_scale(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : __half2float(static_cast<const __half*>(p)[i]);
+}
+// Store into, and or with, CTA `rank`'s copy of the shared variable at `p`.
+RLA_DEVFN void rla_st_dsmem_u32(const void* p, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(rla_mapa(rla_smem_u32(p), rank)), "r"(v) : "memory");
+}
+RLA_DEVFN void rla_or_dsmem_u32(const void* p, uint32_t rank, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(rla_mapa(rla_smem_u32(p), rank)), "r"(v)
+               : "memory");
 }
 RLA_DEVFN double rla_ld_dsmem_f64(const void* p, uint32_t rank) {
   double v;
@@ -439,13 +447,15 @@ RLA_DEVFN double moe_logit(long long key) {
   return key == LLONG_MIN ? __longlong_as_double(LLONG_MAX) : __longlong_as_double(key >= 0 ? key : key ^ LLONG_MAX);
 }
 
-// Softmax and choice from all ranks' partial logits: a warp a token, every
-// CTA of the cluster for itself.  top_k rounds of "the largest that is left,
-// the lowest index of equals"; every round finds an expert, NaN or not.
+// Softmax and choice from all ranks' partial logits: a warp a token.  Every
+// CTA of the cluster chooses for itself where its warps hold all tokens;
+// otherwise (share) each takes every CLUSTER-th token and tells the others.
+// top_k rounds of "the largest that is left, the lowest index of equals";
+// every round finds an expert, NaN or not.
 template <int PER>  // experts of a lane, at least E / 32
-RLA_DEVFN void moe_choose_of(const MoeArgs& g, const double* mine, MoeRoute& r) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int t = warp; t < g.T; t += blockDim.x >> 5) {
+RLA_DEVFN void moe_choose_of(const MoeArgs& g, int rank, bool share, const double* mine, MoeRoute& r) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  for (int t = share ? rank + moe::CLUSTER * warp : warp; t < g.T; t += share ? moe::CLUSTER * warps : warps) {
     double part[PER][moe::CLUSTER];
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -496,21 +506,25 @@ RLA_DEVFN void moe_choose_of(const MoeArgs& g, const double* mine, MoeRoute& r) 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
     if (lane < g.top_k) {
-      r.ids[t * g.top_k + lane] = my_id;
-      r.coef[t * g.top_k + lane] = g.renorm ? __fdividef(p, chosen) : p;
-      atomicOr(&r.mask[my_id], 1u << t);
+      const int at = t * g.top_k + lane;
+      const float coef = g.renorm ? __fdividef(p, chosen) : p;
+      for (int d = share ? 0 : rank; d < (share ? moe::CLUSTER : rank + 1); ++d) {
+        rla_st_dsmem_u32(&r.ids[at], d, static_cast<uint32_t>(my_id));
+        rla_st_dsmem_u32(&r.coef[at], d, __float_as_uint(coef));
+        rla_or_dsmem_u32(&r.mask[my_id], d, 1u << t);
+      }
     }
   }
 }
-RLA_DEVFN void moe_choose(const MoeArgs& g, const double* mine, MoeRoute& r) {
+RLA_DEVFN void moe_choose(const MoeArgs& g, int rank, bool share, const double* mine, MoeRoute& r) {
   if (g.E <= 32)
-    moe_choose_of<1>(g, mine, r);
+    moe_choose_of<1>(g, rank, share, mine, r);
   else if (g.E <= 64)
-    moe_choose_of<2>(g, mine, r);
+    moe_choose_of<2>(g, rank, share, mine, r);
   else if (g.E <= 128)
-    moe_choose_of<4>(g, mine, r);
+    moe_choose_of<4>(g, rank, share, mine, r);
   else
-    moe_choose_of<8>(g, mine, r);
+    moe_choose_of<8>(g, rank, share, mine, r);
 }
 
 // A unit of the gate/up kernel: 16 gate rows and the same 16 up rows of one
@@ -590,10 +604,12 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(32 * moe:
   double* logits = reinterpret_cast<double*>(rings + PART);
   moe_logits<NT>(g, rank, part, logits);
   rla_cluster_sync();
-  moe_choose(g, logits, r);
-  rla_cluster_arrive();  // this CTA has read the others' logits ...
+  const bool share = g.T > WARPS;
+  moe_choose(g, rank, share, logits, r);
+  rla_cluster_arrive();  // this CTA has read the others' logits (and told them its choices) ...
+  if (share) rla_cluster_wait();
   moe_build_lists(r, g.T, g.E, g.top_k);
-  rla_cluster_wait();    // ... and the others this one's: the ring is free
+  if (!share) rla_cluster_wait();  // ... and the others this one's: the ring is free
   rla_fence_proxy_async();  // plain accesses to the ring come before the copies into it
 
   // This CTA's units, and of their stages this warp's run.
