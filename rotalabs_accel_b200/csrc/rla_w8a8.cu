@@ -532,6 +532,15 @@ struct W8Plan {
   size_t smem = 0;
 };
 
+// A pair CTA takes all of its SM's shared memory, although it needs less, so
+// that no other CTA with Tensor Memory sits beside it: a pair holds all 512
+// columns of one SM while it waits for those of the other, and a split cluster
+// of another stream could hold those and wait for the first.  (Split CTAs among
+// themselves cannot: clusters take at least 57 KB for 128 columns or 22 KB for
+// 32, so what fits an SM's shared memory fits its 512 columns.)
+constexpr int kW8PairSmem = 227 * 1024;
+static_assert(sizeof(W8PairShared) + 1024 <= kW8PairSmem, "the ring fits");
+
 // Dynamic shared memory of the split kernel, at most.
 constexpr int kW8SplitSmem = w8::MAX_STAGES * w8::stage_bytes(w8::MAX_BT) + 1024;
 static cudaError_t w8a8_allow_split_smem() {
@@ -626,7 +635,7 @@ static W8Plan w8a8_plan(int64_t M, int64_t N, int64_t K) {
   p.smem = (size_t)p.stages * stage + 1024;
   if (M > 128) {
     const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256), pairs = std::max(1, sms / 2);
-    p.pair = static_cast<double>((pair_tiles + pairs - 1) / pairs) * kb * 0.5 + 1.5 < best;
+    p.pair = static_cast<double>((pair_tiles + pairs - 1) / pairs) * kb * 0.5 + 1.5 < best || p.grid_y > 65535;
   }
   return p;
 }
@@ -659,7 +668,7 @@ static cudaError_t launch_w8a8(const int8_t* x, int64_t ldx, const int8_t* w, in
     if (tiles > INT32_MAX / 2) return cudaErrorInvalidConfiguration;
     const int pairs = static_cast<int>(std::min<int64_t>(tiles, device_sm_count() / 2));
     cfg.gridDim = dim3(2 * pairs);
-    cfg.dynamicSmemBytes = sizeof(W8PairShared) + 1024;
+    cfg.dynamicSmemBytes = kW8PairSmem;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(w8a8_pair_kernel, (int)cfg.dynamicSmemBytes, done);
     if (e != cudaSuccess) return e;

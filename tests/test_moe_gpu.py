@@ -220,6 +220,35 @@ def test_streams_and_graphs(cuda_lib):
         assert all(torch.equal(o, want[a]) for o in outs[0]) and all(torch.equal(o, want[b]) for o in outs[1])
 
 
+def test_two_streams_at_once(cuda_lib):
+    """Eager calls on two streams at the same time, from two host threads,
+    each call with other inputs than the one before it."""
+    import threading
+    import rotalabs_accel_b200 as ra
+    from rotalabs_accel_b200 import _capi
+    problems = [_problem(T, 512, 256, E, seed=T) for T, E in ((1, 8), (12, 32), (30, 16), (70, 8))]
+    want = [ra.int8_moe(*p, top_k=3) for p in problems]
+    torch.cuda.synchronize()
+    wrong, streams = [], [torch.cuda.Stream() for _ in range(2)]
+
+    def work(k):
+        with torch.cuda.stream(streams[k]):
+            for i in range(40):
+                j = (i * (k + 1) + k) % 4
+                if not torch.equal(ra.int8_moe(*problems[j], top_k=3), want[j]):
+                    wrong.append((k, i, j))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and _capi.device_error() == 0
+    # back to back without a wait between: every call's scratch is its own
+    outs = [ra.int8_moe(*problems[i % 4], top_k=3) for i in range(40)]
+    assert all(torch.equal(o, want[i % 4]) for i, o in enumerate(outs))
+
+
 def test_layers_together(cuda_lib):
     """h, xn = add_rmsnorm; the experts and a shared W8A8 block; next norm."""
     import rotalabs_accel_b200 as ra

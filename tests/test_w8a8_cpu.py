@@ -152,3 +152,24 @@ def test_capi_rejects_bad_arguments(lib):
 def test_workspace_size(lib):
     assert lib.rla_w8a8_workspace_size(3, 5, 17) == 8 * 32
     assert lib.rla_w8a8_workspace_size(0, 5, 17) == 0 and lib.rla_w8a8_workspace_size(3, 5, -1) == 0
+
+
+def test_ops_on_meta_tensors(lib):
+    """Shapes and types for tracing, without computing."""
+    from rotalabs_accel_b200 import _capi
+    _capi.torch_ops()
+    e = lambda *s, dt=torch.float16: torch.empty(*s, dtype=dt, device="meta")  # noqa: E731
+    i8, f32 = torch.int8, torch.float32
+    y, h = torch.ops.rla.add_rmsnorm(e(3, 8), e(3, 8), e(8, dt=f32))
+    assert y.shape == h.shape == (3, 8) and y.dtype == h.dtype == torch.float16
+    q, s, h = torch.ops.rla.add_rmsnorm_int8(e(3, 8, dt=torch.bfloat16), e(3, 8, dt=torch.bfloat16), e(8, dt=f32))
+    assert (q.dtype, s.dtype, h.dtype) == (i8, f32, torch.bfloat16) and s.shape == (3,)
+    q, s = torch.ops.rla.swiglu_int8(e(3, 8), e(3, 8))
+    assert (q.dtype, s.dtype) == (i8, f32) and q.shape == (3, 8)
+    y = torch.ops.rla.w8a8_gemm(e(3, 8, dt=i8), e(3, dt=f32), e(5, 8, dt=i8), e(5, dt=f32))
+    assert y.shape == (3, 5) and y.dtype == torch.float16
+    y = torch.ops.rla.moe(e(3, 16), e(4, 16), e(4, 32, 16, dt=i8), e(4, 32), e(4, 32, 16, dt=i8), e(4, 32),
+                          e(4, 16, 32, dt=i8), e(4, 16), 2)
+    assert y.shape == (3, 16) and y.dtype == torch.float16
+    with pytest.raises(RuntimeError, match="Weight shape mismatch"):
+        torch.ops.rla.w8a8_gemm(e(3, 8, dt=i8), e(3, dt=f32), e(5, 9, dt=i8), e(5, dt=f32))

@@ -221,6 +221,17 @@ def test_w8a8_many_tiles(cuda_lib, M, N, K):
     assert _capi.device_error() == 0
 
 
+def test_w8a8_very_many_tokens(cuda_lib):
+    """More token tiles than a grid has rows."""
+    import rotalabs_accel_b200 as ra
+    M, N, K = 8_400_001, 8, 16
+    q, sx, w, sw, _ = _gemm_case(M, N, K, _gen(1))
+    y = ra.int8_gemm_w8a8(q, sx, w, sw)
+    for part in (slice(0, 1000), slice(65535 * 128 - 500, 65535 * 128 + 500), slice(M - 1000, M)):
+        ref, tol = _gemm64(q[part], sx[part], w, sw)
+        assert bool(((y[part].double() - ref).abs() <= tol).all())
+
+
 # rows that TMA cannot address: odd K, odd strides, odd starts
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 5, 15), (17, 130, 257), (70, 33, 4099), (300, 64, 31)])
 def test_w8a8_unaligned(cuda_lib, M, N, K):
@@ -397,6 +408,76 @@ def test_streams_graph_and_ops(cuda_lib):
     up = torch.ops.rla.w8a8_gemm(q, s, mlp.w_up.weight_int8, mlp.w_up.scale)
     q, s = torch.ops.rla.swiglu_int8(gate, up)
     assert torch.equal(torch.ops.rla.w8a8_gemm(q, s, mlp.w_down.weight_int8, mlp.w_down.scale), want[0][0])
+
+
+def test_two_streams_at_once(cuda_lib):
+    """Products of both kernels (CTA pairs and split clusters down to one k
+    block a CTA), norms and SwiGLU on two streams at the same time, from two
+    host threads."""
+    import threading
+    import rotalabs_accel_b200 as ra
+    from rotalabs_accel_b200 import _capi
+    g = _gen(21)
+    cases = [_gemm_case(M, N, K, g) for M, N, K in ((1024, 8192, 1024), (16, 1024, 512), (32, 2048, 1024), (80, 512, 2048),
+                                                    (128, 4096, 512), (2048, 4096, 256))]
+    x = _rand((2048, 4096), g, torch.float16)
+    w = torch.rand(4096, generator=g, device="cuda")
+
+    def all_of(order):
+        out = {}
+        for i in order:
+            out[i] = ra.int8_gemm_w8a8(*cases[i][:4])
+        out["n"] = ra.add_rmsnorm_int8(x, x, w)
+        out["s"] = ra.swiglu_int8(x, x)
+        return out
+
+    want = all_of(range(len(cases)))
+    torch.cuda.synchronize()
+    got, streams = {}, [torch.cuda.Stream() for _ in range(2)]
+
+    def work(k):
+        with torch.cuda.stream(streams[k]):
+            for _ in range(30):
+                got[k] = all_of(range(len(cases)) if k else reversed(range(len(cases))))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        for i in range(len(cases)):
+            assert torch.equal(got[k][i], want[i])
+        assert all(torch.equal(a, b) for n in ("n", "s") for a, b in zip(got[k][n], want[n]))
+    assert _capi.device_error() == 0
+
+
+def test_first_call_inside_a_capture(cuda_lib):
+    """Nothing of a first call (attributes, occupancy) disturbs a capture."""
+    import subprocess
+    import sys
+    code = """
+import torch, rotalabs_accel_b200 as ra
+x = torch.randn(700, 4096, device="cuda").half(); w = torch.ones(4096, device="cuda")
+wt = torch.randint(-9, 9, (512, 4096), dtype=torch.int8, device="cuda"); sw = torch.ones(512, device="cuda") * 1e-3
+r = torch.randn(4, 4096, device="cuda").half()
+wg = torch.randint(-9, 9, (4, 32, 4096), dtype=torch.int8, device="cuda"); sg = torch.ones(4, 32, device="cuda") * 1e-3
+wd = torch.randint(-9, 9, (4, 4096, 32), dtype=torch.int8, device="cuda"); sd = torch.ones(4, 4096, device="cuda") * 1e-3
+torch.cuda.synchronize()
+def run():
+    q, s, h = ra.add_rmsnorm_int8(x, x, w)
+    return (ra.int8_gemm_w8a8(q, s, wt, sw), ra.int8_gemm_w8a8(q[:3], s[:3], wt, sw), *ra.swiglu_int8(x, h),
+            ra.int8_moe(h[:9], r, wg, sg, wg, sg, wd, sd, top_k=2))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = run()
+g.replay(); torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run()))
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
 
 
 def test_rows_around_the_outputs_stay(cuda_lib):
