@@ -26,6 +26,7 @@
 // dispatch, a few microseconds of host time per call.  Same checks, same
 // launch, same result as the op.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -118,6 +119,12 @@ at::Tensor w8a16_gemm_meta(const at::Tensor& x, const at::Tensor& w, const at::T
 // ---------------------------------------------------------------------------
 cudaStream_t stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
+// An output or scratch tensor from torch's allocator, without the dispatcher
+// (a call of the norm makes three).
+at::Tensor empty_on(const at::Device& dev, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, dev, std::nullopt);
+}
+
 int act_dtype(const at::Tensor& t, const char* what) {
   TORCH_CHECK_TYPE(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, what,
                    " must be float16 or bfloat16, got ", t.scalar_type());
@@ -171,12 +178,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_cuda(const at::Tensor& x_in,
   at::Tensor r, h = x_in;
   if (residual.has_value()) {
     r = rows_of(*residual);
-    h = at::empty(x.sizes(), x.options());
+    h = empty_on(dev, x.sizes(), x.scalar_type());
   }
   const int64_t M = x.size(0), K = x.size(1);
-  at::Tensor y = at::empty({M, K}, int8 ? x.options().dtype(at::kChar) : x.options());
+  at::Tensor y = empty_on(dev, {M, K}, int8 ? at::kChar : x.scalar_type());
   at::Tensor scale;
-  if (int8) scale = at::empty({M}, x.options().dtype(at::kFloat));
+  if (int8) scale = empty_on(dev, {M}, at::kFloat);
   const int dt = act_dtype(x, "x");
   const int wdt = weight.scalar_type() == at::kFloat  ? RLA_DTYPE_F32
                   : weight.scalar_type() == at::kHalf ? RLA_DTYPE_F16
@@ -246,8 +253,8 @@ std::tuple<at::Tensor, at::Tensor> swiglu_int8_cuda(const at::Tensor& gate_in, c
   c10::cuda::CUDAGuard guard(dev);
   const at::Tensor gate = rows_of(gate_in), up = rows_of(up_in);
   const int64_t M = gate.size(0), N = gate.size(1);
-  at::Tensor q = at::empty({M, N}, gate.options().dtype(at::kChar));
-  at::Tensor scale = at::empty({M}, gate.options().dtype(at::kFloat));
+  at::Tensor q = empty_on(dev, {M, N}, at::kChar);
+  at::Tensor scale = empty_on(dev, {M}, at::kFloat);
   check_status(rla_swiglu_int8(gate.data_ptr(), row_stride(gate), up.data_ptr(), row_stride(up),
                                act_dtype(gate, "gate"), static_cast<int8_t*>(q.data_ptr()), N,
                                static_cast<float*>(scale.data_ptr()), M, N, stream_of(dev)),
@@ -292,11 +299,11 @@ at::Tensor w8a8_gemm_cuda(const at::Tensor& x_in, const at::Tensor& x_scale_in, 
   at::Tensor bias;
   if (bias_in.has_value()) bias = bias_in->contiguous();
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
-  at::Tensor y = at::empty({M, N}, x.options().dtype(at::kHalf));
+  at::Tensor y = empty_on(dev, {M, N}, at::kHalf);
   if (M == 0 || N == 0) return y;
   at::Tensor ws;
   if (K > 0 && (!rows_aligned(x) || !rows_aligned(w)))
-    ws = at::empty({static_cast<int64_t>(rla_w8a8_workspace_size(M, N, K))}, x.options().dtype(at::kByte));
+    ws = empty_on(dev, {static_cast<int64_t>(rla_w8a8_workspace_size(M, N, K))}, at::kByte);
   check_status(
       rla_w8a8_gemm(static_cast<const int8_t*>(x.data_ptr()), row_stride(x), static_cast<const float*>(x_scale.data_ptr()),
                     static_cast<const int8_t*>(w.data_ptr()), row_stride(w), scale.data_ptr(),
@@ -356,10 +363,10 @@ at::Tensor moe_cuda(const at::Tensor& x_in, const at::Tensor& router_in, const a
   if (!aligned(router)) router = router.clone();
   const at::Tensor s_gate = s_gate_in.contiguous(), s_up = s_up_in.contiguous(), s_down = s_down_in.contiguous();
   const int64_t T = x.size(0), H = x.size(1), I = w_gate.size(1), E = router.size(0);
-  at::Tensor y = at::empty({T, H}, x.options());
+  at::Tensor y = empty_on(dev, {T, H}, at::kHalf);
   const int64_t most = std::min<int64_t>(T, RLA_MOE_MAX_TOKENS);
   const size_t need = rla_moe_workspace_size(most, I, top_k);
-  at::Tensor ws = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
+  at::Tensor ws = empty_on(dev, {static_cast<int64_t>(need)}, at::kByte);
   // longer batches RLA_MOE_MAX_TOKENS rows at a time, in stream order on one scratch
   for (int64_t t0 = 0; t0 < T || t0 == 0; t0 += RLA_MOE_MAX_TOKENS) {
     const int64_t rows = std::min<int64_t>(T - t0, RLA_MOE_MAX_TOKENS);
