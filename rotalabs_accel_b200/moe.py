@@ -6,7 +6,8 @@ reference's ``SwiGLU``, src/rotalabs_accel/kernels/activations.py:140-181, over
 rotalabs-accel has no mixture-of-experts layer.  On CUDA tensors the whole
 layer -- router, choice, gate/up, SwiGLU, down, combination -- is two kernels
 (``rla_moe``) for up to 32 tokens; longer batches run 32 tokens at a time.
-CPU tensors follow the same formulas in torch operations.
+CPU tensors follow the same formulas in torch operations.  For inference: no
+gradients flow.
 """
 
 from __future__ import annotations

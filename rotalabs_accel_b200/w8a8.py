@@ -20,7 +20,7 @@ these join are ``rmsnorm`` (kernels/normalization.py:186-213), ``swiglu_fused``
 ``scale = max|v| / 127``, a zero row gets scale 1, round half to even.
 
 CUDA tensors run the sm_100a kernels (fp16 or bf16 activations); CPU tensors
-the same formulas in torch operations.
+the same formulas in torch operations.  For inference: no gradients flow.
 """
 
 from __future__ import annotations
