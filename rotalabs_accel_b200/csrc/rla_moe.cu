@@ -9,15 +9,16 @@
 // read once, by one warp, and meets all tokens that chose its expert.
 //
 // Stream.  Every warp has a ring of its own in shared memory, filled by bulk
-// tile copies that it issues itself: a stage is 128 bytes of 32 weight rows,
-// in one or two copies.  (One copy a row cost 16 issues, a third of all
-// instructions: 93 us for the case below.)  One CTA of 12 or 16 warps an SM keeps warps x stages x 4 KB on their way
-// (latency x bandwidth needs about 50 KB), through every reduction and change
-// of expert, and no warp waits for another one's data.  (Loads into registers,
-// with the warps of a CTA splitting K and meeting after every 16 rows, took
-// 119 us for one token, 2 of 8 experts of 4096 x 14336.)  The work is cut into
-// stages and every CTA, and every warp of it, gets an equal, contiguous run;
-// a block of rows that spans warps is added up in shared memory.
+// tile copies that it issues itself: a stage is 128 bytes of 32 weight rows, in
+// one or two copies.  One CTA of 12 or 16 warps an SM keeps warps x stages x
+// 4 KB on their way (latency x bandwidth needs about 50 KB), through every
+// reduction and change of expert, and no warp waits for another one's data.
+// The work is cut into stages, and every CTA, and every warp of it, gets an
+// equal, contiguous run; a block of rows that spans warps is added up in shared
+// memory.  Measured for one token, 2 of 8 experts of 4096 x 14336 (54 us at the
+// memory's rate): 67 to 69 us, the gate/up stream at 6.4 TB/s.  Loads into
+// registers with the warps of a CTA splitting K and meeting after every 16 rows
+// took 119 us; copies of single rows, which a warp issues one by one, 93.
 //
 // Products are "swap-AB" tensor-core products like the decode GEMM's: 16
 // weight rows are the rows of an m16n8k16 MMA, the tokens that chose the
