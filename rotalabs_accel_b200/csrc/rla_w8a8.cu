@@ -29,7 +29,6 @@
 // (of a pair's CTA two) for each TMEM lane quarter.  All waits are bounded.
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "rla_common.cuh"
 #include "rla_internal.h"
@@ -124,8 +123,10 @@ RLA_DEVFN void rla_tma2_load_2d(void* smem_dst, const void* desc, uint32_t bar, 
       "l"(desc), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
+// Relaxed: it says that Tensor Memory has been read (tcgen05.wait::ld came before
+// it), and a release would wait for the tile's stores to global memory as well.
 RLA_DEVFN void rla_mbar_arrive_cluster(uint32_t remote) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
 RLA_DEVFN bool rla_mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -164,7 +165,7 @@ struct W8Out {
   int bias_kind;     // 0 none, 1 fp16, 2 fp32
   __half* y;
   int64_t ldy;
-  int vec;  // channels of a store: 8, 4, 2 or 1, as y and its rows are aligned
+  int vec;  // channels of a store: 8, 4 or fewer, as y and its rows are aligned
   int M, N;
 };
 
@@ -180,16 +181,15 @@ RLA_DEVFN __half2 w8a8_values(int sum0, int sum1, float sw, float sx0, float sx1
   return __floats2half2_rn(fmaf(static_cast<float>(sum0) * sw, sx0, bias), fmaf(static_cast<float>(sum1) * sw, sx1, bias));
 }
 
-// 16 rows of 32 channels, out of `buf`, to y: V channels a lane, V rows a store.
-template <int V>
+// 32 rows of 32 channels, out of `buf`, to y: V channels a lane, V rows a store.
+template <int V, typename Word>
 RLA_DEVFN void w8a8_store_rows(const __half* buf, __half* y, int64_t ldy, int rows, int channels) {
-  using Word = typename std::conditional<V == 8, uint4, typename std::conditional<V == 4, uint2,
-               typename std::conditional<V == 2, uint32_t, uint16_t>::type>::type>::type;
+  static_assert(sizeof(Word) == V * sizeof(__half), "");
   const int lane = threadIdx.x & 31;
   const int c = lane % (32 / V) * V;
   const int left = channels - c;
 #pragma unroll 4
-  for (int h = 0; h < 16; h += V) {
+  for (int h = 0; h < 32; h += V) {
     const int r = h + lane / (32 / V);
     if (r >= rows) continue;
     const Word v = *reinterpret_cast<const Word*>(buf + r * 32 + c);
@@ -205,48 +205,62 @@ RLA_DEVFN void w8a8_store_rows(const __half* buf, __half* y, int64_t ldy, int ro
   }
 }
 // One epilogue warp's 32 channels (TMEM lanes) into y: of `cols` token columns
-// 16 from `first` on, and 16 after every `step`.
-// A lane holds one channel, a row of y many: 16 tokens at a time pass through
-// 1 KB of shared memory (`buf`, the warp's own), so that a store instruction is
-// 8 rows of 64 bytes (fewer where y's rows are less than 16-byte aligned), where
-// the lanes' own values would be 16 of one row.  Measured against those stores:
-// 2048x4096x1024 26.7 us to 17.2, 256x8192x128 7.3 to 4.3.
+// 32 from `first` on, and 32 after every `step` (both multiples of 32).
+// A lane holds one channel, a row of y many: 32 tokens at a time pass through
+// 2 KB of shared memory (`buf`, the warp's own), so that a store instruction is
+// 8 rows of 64 bytes (4 where y's rows are 8-byte aligned), where the lanes' own
+// values would be 32 of one row.  Measured against those stores: 2048x4096x1024
+// 26.7 us to 12.5, 256x8192x128 7.3 to 4.8.  Rows of lesser alignment are stored
+// by the lanes: through the buffer 300x2001x64 took 11.8 us where this takes 8.1.
 RLA_DEVFN void w8a8_store_warp(const W8Out& out, uint32_t taddr, int first, int step, int cols, int m0, int n_warp,
                                float sw, float bias, const float* sx, __half* buf) {
   const int lane = threadIdx.x & 31;
   const int channels = out.N - n_warp;
   __half* yp = out.y + (int64_t)(m0 + first) * out.ldy + n_warp;
+  if (out.vec < 4) {
+#pragma unroll 1
+    for (int j = first; j < cols; j = (j & 16) ? j + step - 16 : j + 16) {
+      uint32_t d[16];
+      rla_tmem_ld_32x32b_x16(taddr + j, d);
+      rla_tmem_wait_ld();
+      if (lane < channels) {
+        __half* to = out.y + (int64_t)(m0 + j) * out.ldy + n_warp + lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (j + i < cols) to[i * out.ldy] = w8a8_value(static_cast<int>(d[i]), sw, sx[j + i], bias);
+      }
+    }
+    return;
+  }
 #pragma unroll 1
   for (int j = first; j < cols; j += step, yp += step * out.ldy) {
-    uint32_t d[16];
-    rla_tmem_ld_32x32b_x16(taddr + j, d);
+    uint32_t d[2][16];
+    rla_tmem_ld_32x32b_x16(taddr + j, d[0]);
+    rla_tmem_ld_32x32b_x16(taddr + j + 16, d[1]);  // (may lie behind `cols`, never behind the allocation)
     rla_tmem_wait_ld();
-    __syncwarp();  // the last 16 tokens have left the buffer
+    const int rows = cols - j;
+    __syncwarp();  // the last 32 tokens have left the buffer
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
+    for (int i = 0; i < 32; i += 4) {
+      const uint32_t* di = d[i >> 4] + (i & 15);
       const float4 s4 = *reinterpret_cast<const float4*>(sx + j + i);
-      const __half2 lo = w8a8_values(static_cast<int>(d[i + 0]), static_cast<int>(d[i + 1]), sw, s4.x, s4.y, bias);
-      const __half2 hi = w8a8_values(static_cast<int>(d[i + 2]), static_cast<int>(d[i + 3]), sw, s4.z, s4.w, bias);
+      const __half2 lo = w8a8_values(static_cast<int>(di[0]), static_cast<int>(di[1]), sw, s4.x, s4.y, bias);
+      const __half2 hi = w8a8_values(static_cast<int>(di[2]), static_cast<int>(di[3]), sw, s4.z, s4.w, bias);
       buf[(i + 0) * 32 + lane] = __low2half(lo);
       buf[(i + 1) * 32 + lane] = __high2half(lo);
       buf[(i + 2) * 32 + lane] = __low2half(hi);
       buf[(i + 3) * 32 + lane] = __high2half(hi);
     }
     __syncwarp();
-    const int rows = cols - j;
     if (out.vec == 8)
-      w8a8_store_rows<8>(buf, yp, out.ldy, rows, channels);
-    else if (out.vec == 4)
-      w8a8_store_rows<4>(buf, yp, out.ldy, rows, channels);
-    else if (out.vec == 2)
-      w8a8_store_rows<2>(buf, yp, out.ldy, rows, channels);
+      w8a8_store_rows<8, uint4>(buf, yp, out.ldy, rows, channels);
     else
-      w8a8_store_rows<1>(buf, yp, out.ldy, rows, channels);
+      w8a8_store_rows<4, uint2>(buf, yp, out.ldy, rows, channels);
   }
 }
 
 // bt: token columns of a tile, a multiple of 16 up to MAX_BT.
-__global__ void __launch_bounds__(w8::THREADS)
+__global__ void __launch_bounds__(w8::THREADS, 5)
     w8a8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                       const W8Out out, int num_kb, int stages, int bt, int tmem_cols) {
   const uint32_t stage = w8::stage_bytes(bt);
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(w8::THREADS)
   __shared__ uint64_t full[w8::MAX_STAGES], empty[w8::MAX_STAGES], dfull;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_word;
-  __shared__ __align__(16) float sx_s[w8::MAX_BT];
+  __shared__ __align__(16) float sx_s[w8::MAX_BT + 16];
   __shared__ __align__(16) float sw_s[w8::BR], bias_s[w8::BR];
 
   const int warp = threadIdx.x >> 5;
@@ -352,8 +366,8 @@ __global__ void __launch_bounds__(w8::THREADS)
     rla_tc_fence_after();
     int* part = reinterpret_cast<int*>(ring);  // [bt][128]: every copy and MMA of the ring is done
     if (ok && splits == 1) {
-      w8a8_store_warp(out, tmem + lane_addr, 0, 16, cols, m0, n0 + quarter * 32, sw, bias, sx_s,
-                      reinterpret_cast<__half*>(ring) + quarter * (16 * 32));
+      w8a8_store_warp(out, tmem + lane_addr, 0, 32, cols, m0, n0 + quarter * 32, sw, bias, sx_s,
+                      reinterpret_cast<__half*>(ring) + quarter * (32 * 32));
     } else if (ok) {
 #pragma unroll 1
       for (int j = 0; j < cols; j += 16) {
@@ -427,7 +441,7 @@ struct W8Order {
 struct W8PairShared {
   alignas(1024) uint8_t ring[w8::PAIR_STAGES][2 * 128 * w8::BK];  // 128 channels, then 128 tokens
   alignas(16) float sx[2][w8::PAIR_ROWS];
-  alignas(16) __half buf[8][16 * 32];  // one an epilogue warp
+  alignas(16) __half buf[8][32 * 32];  // one an epilogue warp
   uint64_t full[w8::PAIR_STAGES], empty[w8::PAIR_STAGES], dfull[2], dempty[2], drain;
   uint32_t tmem_base;
   int abort_flag;
@@ -538,23 +552,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::PAIR_THREADS, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int t = threadIdx.x - 64;
     int n_tile = 0;
+    // a thread's channel, and the scale of one of the tokens, for the tile to come
+    // (read while the tile before is stored)
+    float sw = 0.f, bias = 0.f, sx = 0.f;
+    auto fetch = [&](int tile) {
+      if (tile >= tiles) return;
+      int tn, tm;
+      order.at(tile, tn, tm);
+      const int n = tn * w8::PAIR_ROWS + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+      const int m = tm * w8::PAIR_ROWS + t;
+      sw = n < out.N ? w8a8_channel(out.sw, out.sw_f32 ? 2 : 1, n) : 0.f;
+      bias = n < out.N ? w8a8_channel(out.bias, out.bias_kind, n) : 0.f;
+      sx = m < out.M ? out.sx[m] : 0.f;
+    };
+    fetch(pair);
     for (int tile = pair; tile < tiles; tile += pairs, ++n_tile) {
       const int a = n_tile & 1;
       int tn, tm;
       order.at(tile, tn, tm);
-      const int n = tn * w8::PAIR_ROWS + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+      const int n_warp = tn * w8::PAIR_ROWS + static_cast<int>(rank) * 128 + quarter * 32;
       const int m0 = tm * w8::PAIR_ROWS;
       const int cols = min(w8::PAIR_ROWS, out.M - m0);
-      for (int c = t; c < cols; c += 256) sm.sx[a][c] = out.sx[m0 + c];
-      const float sw = n < out.N ? w8a8_channel(out.sw, out.sw_f32 ? 2 : 1, n) : 0.f;
-      const float bias = n < out.N ? w8a8_channel(out.bias, out.bias_kind, n) : 0.f;
-      rla_named_bar_sync(1, 256);
+      const float sw_now = sw, bias_now = bias;
+      sm.sx[a][t] = sx;
+      rla_named_bar_sync(1, 256);  // (nobody still reads what tile - 2 had here)
+      fetch(tile + pairs);
       bool ok = rla_mbar_wait_cluster(&sm.dfull[a], (n_tile >> 1) & 1, RLA_DEVERR_TIMEOUT_ACCUM, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       // (a warp that gave up still meets the others at the barrier above)
       if (!ok) continue;
       rla_tc_fence_after();
-      w8a8_store_warp(out, tmem + lane_addr + a * 256, half * 16, 32, cols, m0, n - lane, sw, bias, sm.sx[a], sm.buf[warp - 2]);
+      w8a8_store_warp(out, tmem + lane_addr + a * 256, half * 32, 64, cols, m0, n_warp, sw_now, bias_now, sm.sx[a], sm.buf[warp - 2]);
       rla_tc_fence_before();
       __syncwarp();
       if (lane == 0) rla_mbar_arrive_cluster(rla_mapa(rla_smem_u32(&sm.dempty[a]), 0));
