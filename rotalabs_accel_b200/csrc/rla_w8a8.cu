@@ -690,8 +690,13 @@ static int w8a8_per_sm(int bt, int stages) { return 228 * 1024 / (stages * w8::s
 //    in one round, 16.4 as 8 in three.
 //  - Slices whose clusters do not all fit at once cost a second round
 //    (300x4096x4096: 21.8 us as 3, 16.1 as 2).
-//  - A round of CTA pairs (256 x 256 tiles) takes about 0.5 us a k block:
-//    2048x4096x4096 pairs 35.2 us, split 43.8; 512x11008x4096 35.3 and 29.9.
+//  - Pairs (256 x 256 tiles) take 2.7 us and, a round, 0.38 us a k block, or
+//    the 3.85 us of an epilogue where that is longer.  Split clusters take 2.6
+//    us, 0.88 of the sum of the above, and 1.1 us a tile of 128 tokens that an
+//    SM stores.  Fitted to 238 sizes (M 144..4096, N 256..28672, K 128..8192)
+//    that both ran, it picks the faster one or one less than 16 % slower:
+//    272x28672x128 pairs 16.5 us, split 9.9; 512x11008x4096 25.6 and 27.3;
+//    2048x4096x1024 12.7 and 18.5; 272x28672x4096 44 and 84.
 static W8Plan w8a8_plan(int64_t M, int64_t N, int64_t K) {
   W8Plan p;
   const int sms = device_sm_count();
@@ -726,7 +731,9 @@ static W8Plan w8a8_plan(int64_t M, int64_t N, int64_t K) {
   p.smem = (size_t)p.stages * stage + 1024;
   if (M > 128) {
     const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256), pairs = std::max(1, sms / 2);
-    p.pair = static_cast<double>((pair_tiles + pairs - 1) / pairs) * kb * 0.5 + 1.5 < best || p.grid_y > 65535;
+    const double rounds = static_cast<double>((pair_tiles + pairs - 1) / pairs);
+    const double stores = static_cast<double>(tiles) * p.bt / 128 / sms;
+    p.pair = 2.7 + rounds * std::max(0.38 * kb, 3.85) < 2.6 + 0.88 * best + 1.1 * stores || p.grid_y > 65535;
   }
   return p;
 }

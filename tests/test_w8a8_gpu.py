@@ -221,6 +221,31 @@ def test_w8a8_many_tiles(cuda_lib, M, N, K):
     assert _capi.device_error() == 0
 
 
+# one tile and several of each kernel, with the slices of K joined and not; the
+# width of a store follows the alignment of y and of its rows
+@pytest.mark.parametrize("M,N,K", [(33, 261, 144), (20, 203, 4112), (130, 5003, 272), (700, 9999, 2064),
+                                   (2049, 6001, 1040)])
+def test_w8a8_output_alignments(cuda_lib, M, N, K):
+    lib = cuda_lib
+    q, sx, w, sw, b = _gemm_case(M, N, K, _gen(M + N), torch.float32, torch.float16)
+    ref, tol = _gemm64(q, sx, w, sw, b)
+    stream = torch.cuda.current_stream().cuda_stream
+    width = (N + 7) // 8 * 8 + 16
+    outs = []
+    for pad, start in ((0, 0), (8, 8), (0, 4), (4, 0), (4, 4), (2, 0), (0, 2), (1, 0), (0, 1), (3, 3)):
+        ld = width + pad
+        buf = torch.full((M + 2, ld), 3.0, dtype=torch.float16, device="cuda")
+        st = lib.rla_w8a8_gemm(q.data_ptr(), K, sx.data_ptr(), w.data_ptr(), K, sw.data_ptr(), 2, b.data_ptr(), 1,
+                               buf.data_ptr() + 2 * (ld + start), ld, M, N, K, None, 0, stream)
+        torch.cuda.synchronize()
+        assert st == 0
+        outs.append(buf[1:1 + M, start:start + N].clone())
+        buf[1:1 + M, start:start + N] = 3.0
+        assert bool((buf == 3.0).all()), (pad, start)
+    assert bool(((outs[0].double() - ref).abs() <= tol).all())
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
 def test_w8a8_very_many_tokens(cuda_lib):
     """More token tiles than a grid has rows."""
     import rotalabs_accel_b200 as ra
