@@ -599,19 +599,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::PAIR_THREADS, 1)
 }
 
 // Rows of K bytes (any alignment, any stride) into rows of `ldd` bytes, zero
-// behind K: what TMA's 16-byte rules need where K or a row stride is odd.
+// behind K: what TMA's 16-byte rules need where K or a row stride is odd.  A
+// thread makes 16 bytes of five aligned words; at the ends of a row, where those
+// would reach beyond it, of single bytes.
 __global__ void w8a8_align_rows_kernel(const int8_t* __restrict__ src, int64_t lds, int8_t* __restrict__ dst, int ldd,
                                        int64_t rows, int K) {
   const int per_row = ldd / 16;
   const int64_t total = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / per_row;
+    // (a 64-bit division takes longer than the copy)
+    const int64_t r = total <= UINT32_MAX ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
     const int k = static_cast<int>(i - r * per_row) * 16;
     const int8_t* p = src + r * lds + k;
-    alignas(16) int8_t v[16];
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3u;
+    alignas(16) uint32_t v[4];
+    if (k >= static_cast<int>(off) && k + 20 - static_cast<int>(off) <= K) {
+      const uint32_t* a = reinterpret_cast<const uint32_t*>(p - off);  // five aligned words, all of this row
+      uint32_t lo = a[0];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = k + j < K ? p[j] : int8_t(0);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t hi = a[j + 1];
+        v[j] = __funnelshift_r(lo, hi, off * 8);
+        lo = hi;
+      }
+    } else {
+      int8_t* b = reinterpret_cast<int8_t*>(v);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) b[j] = k + j < K ? p[j] : int8_t(0);
+    }
     *reinterpret_cast<uint4*>(dst + r * ldd + k) = *reinterpret_cast<const uint4*>(v);
   }
 }
