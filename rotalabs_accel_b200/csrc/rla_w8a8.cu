@@ -608,8 +608,7 @@ __global__ void w8a8_align_rows_kernel(const int8_t* __restrict__ src, int64_t l
   const int64_t total = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    // (a 64-bit division takes longer than the copy)
-    const int64_t r = total <= UINT32_MAX ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
+    const int64_t r = i / per_row;
     const int k = static_cast<int>(i - r * per_row) * 16;
     const int8_t* p = src + r * lds + k;
     const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3u;
