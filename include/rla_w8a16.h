@@ -392,7 +392,8 @@ RLA_API size_t rla_w8a8_workspace_size(int64_t M, int64_t N, int64_t K);
  *
  *     p = softmax(x router^T);  the top_k largest of each token, ties to the
  *     lower index;  c = p, or p / (sum of the chosen p) with renormalize
- *     a = fp16( silu(scale_gate * (w_gate x)) * (scale_up * (w_up x)) )   per chosen expert
+ *     a = silu(scale_gate * (w_gate x)) * (scale_up * (w_up x))   per chosen expert, held
+ *         in two bf16 terms (2^-16 of it is lost, its range is fp32's)
  *     y = fp16( sum over the chosen experts of c * scale_down * (w_down a) )
  *
  *   x       fp16 [T, H], row stride ldx; y fp16 [T, H], row stride ldy

@@ -1,9 +1,13 @@
 // A whole mixture-of-experts layer for up to 32 tokens with int8 expert
 // weights (one scale an output channel), in two kernels:
 //   1. route + gate/up:  p = softmax(x router^T), the top_k largest per token;
-//      a = fp16( silu(sg * (Wg x)) * su * (Wu x) ) for every chosen expert
+//      a = silu(sg * (Wg x)) * su * (Wu x) for every chosen expert
 //   2. down + combine:   y = fp16( sum over the chosen experts of
 //                                  c * sd * (Wd a) ),  c = p or p / sum p
+// a is the sum of two bf16 terms, a = hi + lo with hi = bf16(a), lo = bf16(a -
+// hi): 2^-16 of a at most is lost and fp32's range is kept (a may be far above
+// fp16's 65504 and the scales bring y back).  Tensor-core operands hold no more
+// bits, so the down product is Wd hi + Wd lo in one fp32 sum.
 //
 // Bound by the weights of the experts that some token chose: each byte is
 // read once, by one warp, and meets all tokens that chose its expert.
@@ -16,14 +20,20 @@
 // The work is cut into stages, and every CTA, and every warp of it, gets an
 // equal, contiguous run; a block of rows that spans warps is added up in shared
 // memory.  Measured for one token, 2 of 8 experts of 4096 x 14336 (54 us at the
-// memory's rate): 67 to 69 us, the gate/up stream at 6.4 TB/s.  Loads into
+// memory's rate): 69 us, the gate/up stream at 6.4 TB/s.  Loads into
 // registers with the warps of a CTA splitting K and meeting after every 16 rows
 // took 119 us; copies of single rows, which a warp issues one by one, 93.
 //
 // Products are "swap-AB" tensor-core products like the decode GEMM's: 16
 // weight rows are the rows of an m16n8k16 MMA, the tokens that chose the
-// expert its columns (1, 2 or 4 tiles of 8), int8 -> fp16 in registers, fp32
-// sums.  A column with no token repeats another one's activations and is
+// expert its columns (1, 2 or 4 tiles of 8), int8 -> fp16 (bf16 in the down
+// product) in registers, fp32 sums.  The down product of up to 4 tokens has hi
+// and lo as columns of their own, two of the 8 for each token, and one term
+// would cost as many products; of more tokens, every tile has an MMA for each.
+// What the two terms cost against one of fp16 (of smaller range): 1 token, 2 of
+// 8 experts 67.5 -> 69.4 us, 16 tokens, 8 of 64 71.7 -> 76.0, 32 tokens, 4 of 8
+// (4096 x 2048) 75 -> 84.
+// A column with no token repeats another one's activations and is
 // dropped: columns of a product do not mix, and loads without conditions
 // keep the instructions of a 1 KB piece near the 40 of its conversion.
 //
@@ -36,6 +46,7 @@
 // lower index.
 //
 // Every sum has a fixed order: results are bit-reproducible.
+#include <cuda_bf16.h>
 #include <limits.h>
 
 #include <algorithm>
@@ -93,13 +104,51 @@ struct MoeArgs {
   int scale_f32;
   __half* y;  // [T, H], row stride ldy
   int64_t ldy;
-  __half* a;            // workspace: [T * top_k, I]
+  __nv_bfloat16* a;     // workspace: [T * top_k][hi, lo][I], see moe_place
   MoeTables* tables;    // workspace: the routing, for the second kernel
   int T, H, I, E, top_k, renorm;
 };
 
 RLA_DEVFN float moe_scale(const void* p, int f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : __half2float(static_cast<const __half*>(p)[i]);
+}
+RLA_DEVFN uint32_t rla_and_or(uint32_t a, uint32_t b, uint32_t c) {  // a & b | c
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// int8 -> bf16, four values of a word: bytes 0 and 2 into `even`, 1 and 3 into
+// `odd`.  A byte b >= 0 is (128 + b) - 128, b < 0 is (256 + b) - 256 with
+// 256 + b = 128 + (its low seven bits): both terms are exponent 0x43 with some of the
+// byte's bits in the mantissa, and the difference is exact.
+// (The second is made negative and added: with `sub` of this type the down
+// product of one token issues a third more instructions, 35 us against 30.)
+RLA_DEVFN void rla_i8x4_to_bf2x2(uint32_t w, uint32_t& even, uint32_t& odd) {
+  const uint32_t v = w >> 8;
+  asm("add.rn.bf16x2 %0, %1, %2;"
+      : "=r"(even)
+      : "r"(rla_and_or(w, 0x007f007fu, 0x43004300u)), "r"(rla_and_or(w, 0x00800080u, 0xc300c300u)));
+  asm("add.rn.bf16x2 %0, %1, %2;"
+      : "=r"(odd)
+      : "r"(rla_and_or(v, 0x007f007fu, 0x43004300u)), "r"(rla_and_or(v, 0x00800080u, 0xc300c300u)));
+}
+RLA_DEVFN void rla_mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                  uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Where channel i lies in a row of `a`: the order of the conversion above.
+RLA_DEVFN int moe_place(int i) { return (i & ~3) | (i & 1) << 1 | (i >> 1 & 1); }
+// v = hi + lo.  (The largest finite values would round up to infinity; lo is 0
+// where v is infinite or NaN.)
+RLA_DEVFN void moe_split(float v, __nv_bfloat16& hi, __nv_bfloat16& lo) {
+  hi = __float2bfloat16_rn(v);
+  if (fabsf(__bfloat162float(hi)) == INFINITY) hi = __float2bfloat16_rz(v);
+  const float h = __bfloat162float(hi);
+  lo = __float2bfloat16_rn(fabsf(h) < INFINITY ? v - h : 0.f);
 }
 // Store into, and or with, CTA `rank`'s copy of the shared variable at `p`.
 RLA_DEVFN void rla_st_dsmem_u32(const void* p, uint32_t rank, uint32_t v) {
@@ -257,33 +306,39 @@ RLA_DEVFN int moe_part(int total, int i, int n) {
 // different halves of the 32 banks.
 RLA_DEVFN int moe_row(int g) { return (g >> 1) | ((g & 1) << 2); }
 
-// Activations of a stage.  xp[t]: this lane's of column 8 t + lane / 4 at the
-// stage's first k + 16 * (lane % 4); load(c) reads those of the 64-wide chunk
+// 16-bit activations of a stage.  xp[t]: this lane's of column 8 t + lane / 4
+// at the stage's first k + 16 * (lane % 4); a second term (PARTS = 2) lies
+// `part` elements behind the first.  load(c) reads those of the 64-wide chunk
 // c.  The k order inside the fragments follows the 16-byte pieces
 // (rla_skinny.cu).  `bytes`: the k that are left; behind them zeros meet zeros.
-template <int NT>
+RLA_DEVFN const uint16_t* moe_at(const uint16_t*, const uint16_t* p) { return p; }
+RLA_DEVFN const uint16_t* moe_at(const uint16_t* base, int i) { return base + i; }
+template <int NT, int PARTS>
 struct MoeActs {
-  static constexpr int HELD = NT <= 2 ? 2 : 1;  // chunks in registers
-  uint4 v[HELD][NT][2];
-  template <bool FULL>
-  RLA_DEVFN void load(int c, const __half* const (&xp)[NT], int bytes, int q) {
+  static constexpr int LT = NT * PARTS;
+  static constexpr int HELD = LT <= 2 ? 2 : 1;  // chunks in registers
+  uint4 v[HELD][LT][2];
+  template <bool FULL, class P>
+  RLA_DEVFN void load(int c, const uint16_t* base, const P (&xp)[NT], int part, int bytes, int q) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < LT; ++t) {
       if (FULL || c * 64 + q * 16 < bytes) {
-        v[c % HELD][t][0] = rla_ldg_keep(xp[t] + c * 64);
-        v[c % HELD][t][1] = rla_ldg_keep(xp[t] + c * 64 + 8);
+        const uint16_t* p = moe_at(base, xp[t / PARTS]) + (t % PARTS ? part : 0) + c * 64;
+        v[c % HELD][t][0] = rla_ldg_keep(p);
+        v[c % HELD][t][1] = rla_ldg_keep(p + 8);
       } else {
         v[c % HELD][t][0] = v[c % HELD][t][1] = make_uint4(0, 0, 0, 0);
       }
     }
   }
-  RLA_DEVFN void load_first(const __half* const (&xp)[NT], int bytes, int q) {
+  template <class P>
+  RLA_DEVFN void load_first(const uint16_t* base, const P (&xp)[NT], int part, int bytes, int q) {
     if (bytes >= moe::KB) {
 #pragma unroll
-      for (int c = 0; c < HELD; ++c) load<true>(c, xp, bytes, q);
+      for (int c = 0; c < HELD; ++c) load<true>(c, base, xp, part, bytes, q);
     } else {
 #pragma unroll
-      for (int c = 0; c < HELD; ++c) load<false>(c, xp, bytes, q);
+      for (int c = 0; c < HELD; ++c) load<false>(c, base, xp, part, bytes, q);
     }
   }
 };
@@ -295,8 +350,9 @@ using MoeAcc = float[2][NTM][4];
 // One stage in shared memory at `w`: 32 weight rows x 128 k times NT tiles of
 // 8 columns.  Row g of row tile m is at row m * STEP / 128 + moe_row(g) of the
 // stage, row 8 + g UPPER bytes behind it.  The first chunks of x are loaded.
-template <int NT, int STEP, int UPPER, int NTM>
-RLA_DEVFN void moe_stage(float (&acc)[2][NTM][4], uint32_t w, MoeActs<NT>& x, const __half* const (&xp)[NT], int bytes, int lane) {
+template <int NT, int PARTS, bool BF16, int STEP, int UPPER, int NTM, class P>
+RLA_DEVFN void moe_stage(float (&acc)[2][NTM][4], uint32_t w, MoeActs<NT, PARTS>& x, const uint16_t* base, const P (&xp)[NT],
+                         int part, int bytes, int lane) {
   const int q = lane & 3;
   const int row = moe_row(lane >> 2);
 #pragma unroll
@@ -310,75 +366,88 @@ RLA_DEVFN void moe_stage(float (&acc)[2][NTM][4], uint32_t w, MoeActs<NT>& x, co
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         uint32_t a0, a1, a2, a3;
-        rla_i8x4_to_h2x2(w0[s], a0, a2);
-        rla_i8x4_to_h2x2(w1[s], a1, a3);
+        if constexpr (BF16) {
+          rla_i8x4_to_bf2x2(w0[s], a0, a2);
+          rla_i8x4_to_bf2x2(w1[s], a1, a3);
+        } else {
+          rla_i8x4_to_h2x2(w0[s], a0, a2);
+          rla_i8x4_to_h2x2(w1[s], a1, a3);
+        }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < x.LT; ++t) {
           const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x.v[c % x.HELD][t][0]);
-          rla_mma_16816(acc[m][t], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
+          if constexpr (BF16)
+            rla_mma_16816_bf16(acc[m][t / PARTS], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
+          else
+            rla_mma_16816(acc[m][t / PARTS], a0, a1, a2, a3, xw[2 * s], xw[2 * s + 1]);
         }
       }
     }
     if (c == 0 && x.HELD == 1) {
       if (bytes >= moe::KB)
-        x.template load<true>(1, xp, bytes, q);
+        x.template load<true>(1, base, xp, part, bytes, q);
       else
-        x.template load<false>(1, xp, bytes, q);
+        x.template load<false>(1, base, xp, part, bytes, q);
     }
   }
 }
 
-// `n` stages of one expert from the ring, from k = k0 of `width` on.  Columns
-// are the expert's tokens; the columns behind them repeat its first token and
-// are not used.  row(i): the activations' row of the expert's i-th entry.
+// `n` stages of one expert from the ring, from k = k0 of `width` on.  The
+// columns behind the first `count` repeat column 0 and are not used.  row(i):
+// the activations' row of column i.
 //
 // The activations come from L2, whose latency a warp would meet at every
 // stage: up to 8 tokens they are loaded a stage ahead.  32 rows share them
 // (16 rows of 256 bytes a stage needed twice the loads, and too many
 // registers to load them ahead: 85 us for 8-of-64 at 16 tokens, of which the
 // loads took 14).
-template <int NT, int STEP, int UPPER, int NTM, class Row, class Put>
-RLA_DEVFN bool moe_run_tiles(float (&acc)[2][NTM][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
-                             volatile int* abort_flag, const Row& row, const Put& put) {
+template <int NT, int PARTS, bool BF16, int STEP, int UPPER, int NTM, class Row, class Put>
+RLA_DEVFN bool moe_run_tiles(float (&acc)[2][NTM][4], MoeRing& ring, int n, int k0, int width, int part, int count,
+                             int lane, volatile int* abort_flag, const uint16_t* base, const Row& row, const Put& put) {
+  constexpr bool AHEAD = NT * PARTS == 1;
   const int q = lane & 3;
-  const __half* xp[NT];
+  using P = decltype(row(0));
+  P xp[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int col = t * 8 + (lane >> 2);
     xp[t] = row(col < count ? col : 0) + k0 + q * 16;
   }
   int bytes = width - k0;  // from this stage's k on
-  MoeActs<NT> x;
-  if (NT == 1) x.load_first(xp, bytes, q);
+  MoeActs<NT, PARTS> x;
+  if constexpr (AHEAD) x.load_first(base, xp, part, bytes, q);
 #pragma unroll 1
   for (int i = 0; i < n; ++i) {
-    MoeActs<NT> ahead;
-    if constexpr (NT == 1) {
-      const __half* next[1] = {xp[0] + moe::KB};
-      if (i + 1 < n) ahead.load_first(next, bytes - moe::KB, q);
+    MoeActs<NT, PARTS> ahead;
+    if constexpr (AHEAD) {
+      const P next[1] = {xp[0] + moe::KB};
+      if (i + 1 < n) ahead.load_first(base, next, part, bytes - moe::KB, q);
     } else {
-      x.load_first(xp, bytes, q);
+      x.load_first(base, xp, part, bytes, q);
     }
     uint32_t w;
     if (!ring.wait(abort_flag, w)) return false;
-    moe_stage<NT, STEP, UPPER>(acc, w, x, xp, bytes, lane);
+    moe_stage<NT, PARTS, BF16, STEP, UPPER>(acc, w, x, base, xp, part, bytes, lane);
     __syncwarp();
     put();
 #pragma unroll
     for (int t = 0; t < NT; ++t) xp[t] += moe::KB;
     bytes -= moe::KB;
-    if (NT == 1) x = ahead;
+    if constexpr (AHEAD) x = ahead;
   }
   return true;
 }
-template <int STEP, int UPPER, int NTM, class Row, class Put>
-RLA_DEVFN bool moe_run(float (&acc)[2][NTM][4], MoeRing& ring, int n, int k0, int width, int count, int lane,
-                       volatile int* abort_flag, const Row& row, const Put& put) {
+// The tiles that `count` columns need, of PARTS terms each.
+template <int PARTS, bool BF16, int STEP, int UPPER, int NTM, class Row, class Put>
+RLA_DEVFN bool moe_run(float (&acc)[2][NTM][4], MoeRing& ring, int n, int k0, int width, int part, int count, int lane,
+                       volatile int* abort_flag, const uint16_t* base, const Row& row, const Put& put) {
   if constexpr (NTM == 4)
-    if (count > 16) return moe_run_tiles<4, STEP, UPPER>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+    if (count > 16)
+      return moe_run_tiles<4, PARTS, BF16, STEP, UPPER>(acc, ring, n, k0, width, part, count, lane, abort_flag, base, row, put);
   if constexpr (NTM >= 2)
-    if (count > 8) return moe_run_tiles<2, STEP, UPPER>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
-  return moe_run_tiles<1, STEP, UPPER>(acc, ring, n, k0, width, count, lane, abort_flag, row, put);
+    if (count > 8)
+      return moe_run_tiles<2, PARTS, BF16, STEP, UPPER>(acc, ring, n, k0, width, part, count, lane, abort_flag, base, row, put);
+  return moe_run_tiles<1, PARTS, BF16, STEP, UPPER>(acc, ring, n, k0, width, part, count, lane, abort_flag, base, row, put);
 }
 template <int NTM>
 RLA_DEVFN void moe_zero(float (&acc)[2][NTM][4]) {
@@ -553,12 +622,11 @@ RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int g
     for (int j = 0; j < 2; ++j) {
       const int col = t * 8 + 2 * q + j;
       if (col < count) {
-        __half* to = g.a + (int64_t)r.entry[first + col] * g.I + group * 16 + moe_row(lane >> 2);
+        __nv_bfloat16* to = g.a + (int64_t)r.entry[first + col] * 2 * g.I + group * 16 + moe_place(moe_row(lane >> 2));
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           const float gate = acc[m][t][j] * sc.gate[m], up = acc[m][t][2 + j] * sc.up[m];
-          // the down product's tensor-core operand is fp16: one rounding
-          to[m * 8] = __float2half_rn(__fdividef(gate, 1.0f + __expf(-gate)) * up);
+          moe_split(__fdividef(gate, 1.0f + __expf(-gate)) * up, to[m * 8], to[g.I + m * 8]);
         }
       }
     }
@@ -659,8 +727,10 @@ __global__ void __cluster_dims__(moe::CLUSTER, 1, 1) __launch_bounds__(32 * moe:
       const int e = r.active[ca], first = r.begin[e];
       const int n = min(per - cs, left);
       scales.load(g, e, cg, lane);  // (read before the products, used after them)
-      ok = moe_run<1024, moe::SLOT / 2>(acc, ring, n, cs * moe::KB, g.H, __popc(r.mask[e]), lane, &r.abort_flag,
-                                        [&](int i) { return g.x + r.token[first + i] * g.ldx; }, put);
+      ok = moe_run<1, false, 1024, moe::SLOT / 2>(acc, ring, n, cs * moe::KB, g.H, 0, __popc(r.mask[e]), lane,
+                                                  &r.abort_flag, nullptr, [&](int i) {
+                                                    return reinterpret_cast<const uint16_t*>(g.x + r.token[first + i] * g.ldx);
+                                                  }, put);
       left = ok ? left - n : 0;
       cs += n;
       if (!ok) {
@@ -763,6 +833,7 @@ __global__ void __launch_bounds__(32 * moe::warps(NT), 1)
   bool ok = true;
   const int values = g.T * moe::ROWS;
   float* own = sums + warp * values;
+  const uint16_t* a = reinterpret_cast<const uint16_t*>(g.a);  // (at most 2^28 elements: 32-bit indices)
   for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
     for (int p = lane; p < values; p += 32) own[p] = 0.f;
     int ca = a0, cs = s0, left = n;
@@ -776,16 +847,28 @@ __global__ void __launch_bounds__(32 * moe::warps(NT), 1)
             moe_scale(g.s_down, g.scale_f32, (int64_t)e * g.H + min(b * moe::ROWS + gr + i * 8, g.H - 1));
       MoeAcc<NT> acc;
       moe_zero(acc);
-      ok = moe_run<2048, 1024>(acc, ring, m, cs * moe::KB, g.I, count, lane, &r.abort_flag,
-                               [&](int i) { return g.a + (int64_t)r.entry[first + i] * g.I; }, put);
+      // up to 4 tokens: columns 2 i and 2 i + 1 are the terms of entry i
+      const bool paired = count <= 4;
+      if (paired)
+        ok = moe_run_tiles<1, 1, true, 2048, 1024>(
+            acc, ring, m, cs * moe::KB, g.I, 0, 2 * count, lane, &r.abort_flag, a,
+            [&](int i) { return (r.entry[first + (i >> 1)] * 2 + (i & 1)) * g.I; }, put);
+      else
+        ok = moe_run<2, true, 2048, 1024>(acc, ring, m, cs * moe::KB, g.I, g.I, count, lane, &r.abort_flag, a,
+                                          [&](int i) { return r.entry[first + i] * 2 * g.I; }, put);
       if (!ok) break;
+      if (paired) {  // both terms into the column of the lane's first
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i >> 1][0][2 * (i & 1)] += acc[i >> 1][0][2 * (i & 1) + 1];
+      }
       __syncwarp();  // the zeros, or another expert's sums, are in place
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t * 8 >= count) break;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int col = t * 8 + 2 * q + j;
+          if (j == 1 && paired) break;
+          const int col = paired ? q : t * 8 + 2 * q + j;
           if (col < count) {
             const float c = r.coef[r.entry[first + col]];
             float* v = own + r.token[first + col] * moe::ROWS + gr;
@@ -916,7 +999,7 @@ extern "C" {
 size_t rla_moe_workspace_size(int64_t T, int64_t I, int64_t top_k) {
   if (T <= 0 || I <= 0 || top_k <= 0 || T > RLA_MOE_MAX_TOKENS || top_k > RLA_MOE_MAX_TOP_K) return 0;
   const size_t n = (size_t)T * (size_t)top_k;
-  return rla::moe_up256(n * (size_t)I * 2) + rla::moe_up256(sizeof(rla::MoeTables));
+  return rla::moe_up256(n * (size_t)I * 4) + rla::moe_up256(sizeof(rla::MoeTables));
 }
 
 int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate, const void* scale_gate,
@@ -949,10 +1032,10 @@ int rla_moe(const void* x, int64_t ldx, const void* router, const int8_t* w_gate
   }
   char* ws = static_cast<char*>(workspace);
   const size_t n = (size_t)T * (size_t)top_k;
-  const size_t a_bytes = moe_up256(n * (size_t)I * 2);
+  const size_t a_bytes = moe_up256(n * (size_t)I * 4);
   const MoeArgs g{static_cast<const __half*>(x), ldx, static_cast<const __half*>(router), w_gate, w_up, w_down,
                   scale_gate, scale_up, scale_down, scale_dtype == RLA_DTYPE_F32 ? 1 : 0, static_cast<__half*>(y), ldy,
-                  reinterpret_cast<__half*>(ws), reinterpret_cast<MoeTables*>(ws + a_bytes), (int)T, (int)H, (int)I, (int)E, (int)top_k,
+                  reinterpret_cast<__nv_bfloat16*>(ws), reinterpret_cast<MoeTables*>(ws + a_bytes), (int)T, (int)H, (int)I, (int)E, (int)top_k,
                   renormalize ? 1 : 0};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = moe_tiles((int)T) == 1   ? launch_moe<1>(g, s)

@@ -59,6 +59,9 @@ def int8_moe(x: torch.Tensor, router_weight: torch.Tensor, w_gate: torch.Tensor,
             all fp32 or all fp16.
         renormalize: ``c = p / sum of the chosen p`` (else ``c = p``).
 
+    Sums are fp32; ``silu(gate) * up`` keeps fp32's range and 16 bits (CUDA:
+    two bf16 terms; CPU: fp32).
+
     Returns ``(..., H)``, fp16 for CUDA inputs, ``x.dtype`` for CPU inputs.
     On CUDA: E <= 256, top_k <= 32, H and I multiples of 16.
     """
