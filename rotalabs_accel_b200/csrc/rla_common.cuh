@@ -92,7 +92,8 @@ RLA_DEVFN __half rla_swiglu(float gate, float up) {
 // ---------------------------------------------------------------------------
 // Global loads
 // ---------------------------------------------------------------------------
-// Streaming 16-byte load of weights: read once, keep out of L1.
+// Streaming 16-byte load of weights: read once, keep out of L1.  Non-coherent:
+// only for what no kernel that may still run when this one starts writes.
 RLA_DEVFN uint4 rla_ldg_stream(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -101,9 +102,12 @@ RLA_DEVFN uint4 rla_ldg_stream(const void* p) {
   return v;
 }
 // 16-byte load of activations: shared by every warp of the CTA, keep in L1.
+// A coherent load: under programmatic dependent launch the kernel that writes
+// the activations may run beside this one's beginning, and the non-coherent
+// form asks for data that nobody writes while the kernel is resident.
 RLA_DEVFN uint4 rla_ldg_keep(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;

@@ -139,7 +139,10 @@ cudaError_t launch_swiglu(const void* gate, const void* up, int64_t ld, void* y,
 // (kernels/normalization.py:66-101): per row, the mean of x^2 in fp32,
 // rrms = rsqrt(mean + eps), y = fp16(x * rrms * w) computed in fp32.  One CTA
 // per row; 16-byte loads when the row is aligned.  Launched with
-// programmatic dependent launch, so the next GEMM's prologue overlaps it.
+// programmatic dependent launch, so the next GEMM's prologue overlaps it.  (x
+// is not declared __restrict__: the compiler would read it through the
+// non-coherent path, and the kernel before this one may still be writing it
+// when this one becomes resident.)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float load_weight(const void* w, int dtype, int k) {
   return dtype == RLA_DTYPE_F32  ? static_cast<const float*>(w)[k]
@@ -147,8 +150,8 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, int k) {
                                   : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[k]);
 }
 
-__global__ void rmsnorm_rows_kernel(const __half* __restrict__ x, int64_t ldx, const void* __restrict__ weight,
-                                    int weight_dtype, float eps, __half* __restrict__ y, int64_t ldy, int K,
+__global__ void rmsnorm_rows_kernel(const __half* x, int64_t ldx, const void* __restrict__ weight,
+                                    int weight_dtype, float eps, __half* y, int64_t ldy, int K,
                                     int vec) {
   // Programmatic dependent launch: the GEMM that follows (the MLP block's
   // gate/up projection) may start now and stream its weights while this
