@@ -89,6 +89,17 @@ RLA_DEVFN __half rla_swiglu(float gate, float up) {
   return __float2half_rn(__fdividef(gu.x, 1.0f + __expf(-gu.x)) * gu.y);
 }
 
+// silu(f) * u in fp32 where f <= -87: 1 + e^-f is beyond the range of the
+// quotients above, and silu(f) = f e^f (to 2^-125) itself below fp32's, but a
+// large u brings the product back: -88 times 1e38 is -53.  So e^f is taken as the
+// square of e^(f / 2), one factor on each side of u.
+RLA_DEVFN float rla_silu_mul_far(float f, float u) {
+  const float t = f * 0.72134752f;  // log2(e) / 2
+  float h;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(h) : "f"(t));
+  return f * h * u * h;
+}
+
 // ---------------------------------------------------------------------------
 // Global loads
 // ---------------------------------------------------------------------------

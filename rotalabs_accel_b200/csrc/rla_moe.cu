@@ -664,7 +664,8 @@ RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int g
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           const float gate = acc[m][t][j] * sc.gate[m], up = acc[m][t][2 + j] * sc.up[m];
-          moe_split(__fdividef(gate, 1.0f + __expf(-gate)) * up, to[m * 8], to[g.I + m * 8]);
+          const float a = gate < -87.f ? rla_silu_mul_far(gate, up) : __fdividef(gate, 1.0f + __expf(-gate)) * up;
+          moe_split(a, to[m * 8], to[g.I + m * 8]);
         }
       }
     }

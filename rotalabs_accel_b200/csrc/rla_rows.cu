@@ -16,8 +16,8 @@
 // A row is held in registers (EPT elements a thread) between the reduction
 // and the output, so nothing is read twice up to 1024 * 32 = 32768 columns;
 // longer rows are read a second time.  Many rows run through persistent CTAs
-// that have the next rows on their way while one is reduced (below).  SwiGLU comes near the issue limit too
-// (some 11 instructions an element, two of them on the special-function unit), so
+// that have the next rows on their way while one is reduced (below).  SwiGLU has
+// some 11 instructions an element, two of them on the special-function unit, so
 // the quantization is one FMA: p * (127 / max) + 1.5 * 2^23 rounds to nearest
 // even in the last bit of the sum, whose low byte is q.
 #include <cuda_bf16.h>
@@ -95,21 +95,46 @@ RLA_DEVFN void rows_load_weight(const void* w, int dtype, int k, float (&out)[V]
   }
 }
 
-// silu(f) = f / (1 + e^-f).  The approximations' few ulp are far below the
-// 8-bit step, and move the scale by less than 1e-6 of itself; flushing
-// subnormals changes only results below 1e-36 (and saves the instructions that
-// would scale them).
+// silu(f) = f / (1 + e^-f) for f > -87 (so that nothing is flushed: e^87 < 2^126; saving
+// the instructions that scale subnormals).  Its relative error is at most 2^-20, and for
+// negative f also |f| 2^-23.7 from the rounding of f log2(e) and of log2(e): far below
+// the 8-bit step, and up to 6e-6 of a scale that comes from a gate of -87.
 RLA_DEVFN float rows_silu(float f) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(f * -1.44269504f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return f * r;
 }
+// v = silu(a) * b; `low`: the lowest a so far, in two 16-bit halves.
+template <typename T>
+struct RowsPair {
+  using type = __half2;
+};
+template <>
+struct RowsPair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
 template <typename T, int V>
-RLA_DEVFN void rows_swiglu(const RowVec<T, V>& a, const RowVec<T, V>& b, float (&p)[V]) {
+RLA_DEVFN void rows_swiglu(const RowVec<T, V>& a, const RowVec<T, V>& b, float (&p)[V], typename RowsPair<T>::type& low) {
+  using Pair = typename RowsPair<T>::type;
+#pragma unroll
+  for (int i = 0; i < V; ++i) p[i] = rows_silu(rows_to_f(a.v[i])) * rows_to_f(b.v[i]);
+#pragma unroll
+  for (int i = 0; i < V; i += 2) low = __hmin2(low, Pair{a.v[i], a.v[V > 1 ? i + 1 : i]});
+}
+// Gates below -87 are rare, and v there is 0 so far: the callers look once at the
+// lowest and set those v (a test at each took 1.7 us of 26 at 2048 x 11008).
+template <typename Pair>
+RLA_DEVFN bool rows_far(const Pair& low) {
+  return __builtin_expect(fminf(rows_to_f(low.x), rows_to_f(low.y)) < -87.f, 0);
+}
+template <typename T, int V>
+RLA_DEVFN void rows_swiglu_far(const RowVec<T, V>& a, const RowVec<T, V>& b, float (&p)[V], float& top) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    p[i] = rows_silu(rows_to_f(a.v[i])) * rows_to_f(b.v[i]);
+    const float f = rows_to_f(a.v[i]);
+    if (f < -87.f) p[i] = rla_silu_mul_far(f, rows_to_f(b.v[i]));
+    top = rows_max_nan(top, fabsf(p[i]));
   }
 }
 // The residual stream has the activations' type: one rounding, and the norm is
@@ -138,7 +163,11 @@ RLA_DEVFN void rows_vector(const RowsArgs& g, int64_t row, int k, bool store, fl
   using Vec = RowVec<T, V>;
   const Vec a = *reinterpret_cast<const Vec*>(static_cast<const T*>(g.a) + row * g.lda + k);
   if constexpr (OP == kRowsSwiGLUInt8) {
-    rows_swiglu(a, *reinterpret_cast<const Vec*>(static_cast<const T*>(g.b) + row * g.ldb + k), p);
+    const Vec b = *reinterpret_cast<const Vec*>(static_cast<const T*>(g.b) + row * g.ldb + k);
+    typename RowsPair<T>::type low{rows_from_f<T>(0.f), rows_from_f<T>(0.f)};
+    rows_swiglu(a, b, p, low);
+    float unused = 0.f;
+    if (rows_far(low)) rows_swiglu_far(a, b, p, unused);
   } else {
     Vec h = a;
     if (g.b) {
@@ -337,13 +366,14 @@ __global__ void __launch_bounds__(MAXT, CTAS) rows_stream_kernel(const RowsArgs 
     const uint8_t* from = rows_ring + (size_t)s * 2 * row_bytes;
     float p[NV][8];
     float ss = 0.f, top = 0.f;
+    typename RowsPair<T>::type low{rows_from_f<T>(0.f), rows_from_f<T>(0.f)};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int k = (j * blockDim.x + tid) * 8;
       if (k >= g.K) continue;
       const Vec a = *reinterpret_cast<const Vec*>(from + k * 2);
       if constexpr (OP == kRowsSwiGLUInt8) {
-        rows_swiglu(a, *reinterpret_cast<const Vec*>(from + row_bytes + k * 2), p[j]);
+        rows_swiglu(a, *reinterpret_cast<const Vec*>(from + row_bytes + k * 2), p[j], low);
       } else {
         Vec h = a;
         if (two) {
@@ -356,6 +386,17 @@ __global__ void __launch_bounds__(MAXT, CTAS) rows_stream_kernel(const RowsArgs 
       if constexpr (OP != kRowsNorm) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = rows_max_nan(top, fabsf(p[j][i]));
+      }
+    }
+    if constexpr (OP == kRowsSwiGLUInt8) {
+      if (rows_far(low)) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int k = (j * blockDim.x + tid) * 8;
+          if (k < g.K)
+            rows_swiglu_far(*reinterpret_cast<const Vec*>(from + k * 2),
+                            *reinterpret_cast<const Vec*>(from + row_bytes + k * 2), p[j], top);
+        }
       }
     }
     rows_reduce_warp<OP>(ss, top);

@@ -17,6 +17,7 @@ import torch
 from . import _capi
 from .gemm import _as_2d_fp16
 from .quantization import quantize_weight_per_channel
+from .w8a8 import _silu_mul
 
 
 def int8_moe_torch(x: torch.Tensor, router_weight: torch.Tensor, w_gate: torch.Tensor, scale_gate: torch.Tensor,
@@ -38,7 +39,7 @@ def int8_moe_torch(x: torch.Tensor, router_weight: torch.Tensor, w_gate: torch.T
         xe = x2[token]
         gate = xe @ w_gate[e].float().t() * scale_gate[e].float()
         up = xe @ w_up[e].float().t() * scale_up[e].float()
-        a = torch.nn.functional.silu(gate) * up
+        a = _silu_mul(gate, up)
         y[token] += chosen[token, place].float().unsqueeze(1) * (a @ w_down[e].float().t() * scale_down[e].float())
     return y.to(x.dtype).view(x.shape)
 

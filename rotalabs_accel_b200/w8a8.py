@@ -45,6 +45,12 @@ def _quantize_rows(v: torch.Tensor):
     return torch.nan_to_num(q, nan=0.0).to(torch.int8), scale
 
 
+def _silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """``silu(gate) * up``, rounded once to fp32 (``silu`` of a gate below -88
+    is beyond fp32's range; times a large ``up`` it may not be)."""
+    return (torch.nn.functional.silu(gate.double()) * up.double()).float()
+
+
 def _rows(x: Optional[torch.Tensor]):
     """``(..., K)`` as ``(rows, K)`` (None stays None)."""
     return None if x is None else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
@@ -135,7 +141,7 @@ def swiglu_int8(gate: torch.Tensor, up: torch.Tensor):
     if gate.is_cuda:
         q, s = _capi.torch_ops().swiglu_int8(_rows(gate), _rows(up))
         return q.view(gate.shape), s.view(gate.shape[:-1])
-    return _quantize_rows(torch.nn.functional.silu(gate.float()) * up.float())
+    return _quantize_rows(_silu_mul(gate, up))
 
 
 def int8_gemm_w8a8(x_int8: torch.Tensor, x_scale: torch.Tensor, weight_int8: torch.Tensor, scale: torch.Tensor,
