@@ -26,7 +26,15 @@
 //
 // Warp roles: warp 0 TMA producer (a ring of 128-byte-wide k blocks, 128-byte
 // swizzle), warp 1 TMEM allocation and MMA issue, then the epilogue's warps, one
-// (of a pair's CTA two) for each TMEM lane quarter.  All waits are bounded.
+// (of a pair's CTA two) for each TMEM lane quarter.
+//
+// Waits.  Every mbarrier wait is bounded; after one that gave up, the CTAs still
+// see all their copies land and their MMAs end before they leave.  The cluster's
+// barriers and tcgen05.alloc have no limit.  A barrier is reached by every
+// warp whatever its waits returned.  An allocation waits for CTAs of the same
+// SM to leave: this library's kernels cannot wait for one another in a circle
+// (see kW8PairSmem); a library's kernel on another stream that holds Tensor
+// Memory on one SM while it waits for another SM's is not excluded.
 #include <algorithm>
 #include <atomic>
 
@@ -85,6 +93,14 @@ RLA_DEVFN int4 rla_ld_cluster_int4(uint32_t remote) {
                : "r"(remote)
                : "memory");
   return v;
+}
+
+RLA_DEVFN void rla_st_cluster_u32(uint32_t remote, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+// As if `bytes` of a copy that counts on the barrier had arrived.
+RLA_DEVFN void rla_mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(rla_smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // ---- CTA pairs (cta_group::2): the even CTA of the cluster leads ----
@@ -323,9 +339,10 @@ __global__ void __launch_bounds__(w8::THREADS, 5)
         rla_tma_load_2d(slot + w8::BR * w8::BK, &tmap_x, &full[s], (kb0 + i) * w8::BK, m0);
         issued = i + 1;
       }
-      if (*abort_flag)  // do not leave while copies may still land in shared memory
-        for (int i = max(0, issued - stages); i < issued; ++i)
-          rla_mbar_wait(&full[i % stages], (i / stages) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
+      // do not leave while copies may still land in shared memory: the MMA warp
+      // waits for them too, but may give up after this warp has issued its last
+      for (int i = max(0, issued - stages); i < issued; ++i)
+        rla_mbar_wait(&full[i % stages], (i / stages) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -444,8 +461,25 @@ struct W8PairShared {
   alignas(16) __half buf[8][32 * 32];  // one an epilogue warp
   uint64_t full[w8::PAIR_STAGES], empty[w8::PAIR_STAGES], dfull[2], dempty[2], drain;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, issued;            // issued: k blocks that this CTA's copies were issued for
+  int peer_abort_flag, peer_issued;  // the other CTA's, at the end
 };
+// After a wait that gave up, by the leader when both CTAs are through: all
+// copies in flight land.  Both CTAs' bytes count on the leader's barriers, which
+// expect them for the blocks that the leader issued (n0); the other CTA may have
+// stopped before it (n1 < n0), and its bytes are taken as arrived, or after it, and
+// they are expected now.  (It is at most a ring ahead: it waits for the leader's commits.)
+RLA_DEVFN void w8a8_pair_drain(W8PairShared& sm, uint32_t half) {
+  constexpr int STAGES = w8::PAIR_STAGES;
+  const int n0 = sm.issued, n1 = sm.peer_issued, last = max(n0, n1);
+  for (int i = max(0, last - STAGES); i < last; ++i) {
+    uint64_t* bar = &sm.full[i % STAGES];
+    if (i >= n0) rla_mbar_arrive_expect_tx(bar, 2 * half);
+    if (i >= n1) rla_mbar_complete_tx(bar, 2 * half);
+  }
+  for (int i = max(0, last - STAGES); i < last; ++i)
+    rla_mbar_wait_cluster(&sm.full[i % STAGES], (i / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
+}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::PAIR_THREADS, 1)
     w8a8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
@@ -475,6 +509,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::PAIR_THREADS, 1)
     }
     rla_mbar_init(&sm.drain, 1);
     sm.abort_flag = 0;
+    sm.issued = 0;
     rla_fence_barrier_init();
   }
   if (warp == 1) {
@@ -510,9 +545,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::PAIR_THREADS, 1)
           rla_tma2_load_2d(sm.ring[s] + HALF, &tmap_x, bar, kb * w8::BK, m0);
         }
       }
-      if (*abort_flag && rank == 0)  // both CTAs' copies count here, and both stay until the end
-        for (int i = max(0, it - STAGES); i < it; ++i)
-          rla_mbar_wait_cluster(&sm.full[i % STAGES], (i / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
+      sm.issued = it;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -590,8 +623,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(w8::PAIR_THREADS, 1)
   }
   rla_tc_fence_before();
   __syncthreads();
-  // both CTAs are through: nothing reads or writes the other's shared memory or TMEM any more
+  if (threadIdx.x == 0) {
+    rla_st_cluster_u32(rla_mapa(rla_smem_u32(&sm.peer_abort_flag), rank ^ 1u), static_cast<uint32_t>(*abort_flag));
+    rla_st_cluster_u32(rla_mapa(rla_smem_u32(&sm.peer_issued), rank ^ 1u), static_cast<uint32_t>(sm.issued));
+  }
+  __syncwarp();
+  // both CTAs are through: without a wait that gave up, nothing reads or writes
+  // the other's shared memory or TMEM any more
   rla_cluster_sync();
+  if (*abort_flag || sm.peer_abort_flag) {  // (the same in all threads of both)
+    if (rank == 0 && threadIdx.x == 0) w8a8_pair_drain(sm, HALF);
+    __syncwarp();
+    rla_cluster_sync();
+  }
   if (warp == 1) {
     rla_tc_fence_after();
     rla_tmem2_dealloc(tmem, 512);
