@@ -188,11 +188,10 @@ __global__ void __launch_bounds__(sk::THREADS, 1)
         if (c0 == c_count) { c0 = 0; ++rb; }
         issued = it + 1;
       }
-      if (*abort_flag) {
-        // Let the copies already issued land before the CTA exits.
-        for (int it = max(0, issued - STAGES); it < issued; ++it)
-          rla_mbar_wait(&full[it % STAGES], (it / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
-      }
+      // Let the copies already issued land before the CTA exits (a consumer
+      // may give up after this warp has issued its last).
+      for (int it = max(0, issued - STAGES); it < issued; ++it)
+        rla_mbar_wait(&full[it % STAGES], (it / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
     }
     return;
   }

@@ -124,11 +124,10 @@ __global__ void __launch_bounds__(tc::THREADS, 1)
         rla_tma_load_2d(sm.w[s], &tmap_w, &sm.full[s], kb * tc::BK, n0);
         issued_until = kb + 1;
       }
-      if (*abort_flag) {
-        // Do not leave the CTA while our copies may still land in shared memory.
-        for (int kb = max(0, issued_until - STAGES); kb < issued_until; ++kb)
-          rla_mbar_wait(&sm.full[kb % STAGES], (kb / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
-      }
+      // Do not leave the CTA while our copies may still land in shared memory
+      // (another warp may give up after this one has issued its last).
+      for (int kb = max(0, issued_until - STAGES); kb < issued_until; ++kb)
+        rla_mbar_wait(&sm.full[kb % STAGES], (kb / STAGES) & 1, RLA_DEVERR_TIMEOUT_TMA_FULL, nullptr);
     }
     __syncwarp();
   } else if (warp == 1) {

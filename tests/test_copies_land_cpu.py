@@ -24,12 +24,13 @@ def _kernel(code, name):
     return code[start:end if end > 0 else None]
 
 
-@pytest.mark.parametrize("name,kernel", [("rla_w8a8.cu", "w8a8_split_kernel")])
+@pytest.mark.parametrize("name,kernel", [("rla_w8a8.cu", "w8a8_split_kernel"), ("rla_tc.cu", "w8a16_tc_kernel"),
+                                         ("rla_stream.cu", "w8a16_stream_kernel")])
 def test_the_producer_waits_for_its_last_copies(name, kernel):
     body = _kernel(_code(name), kernel)
     drain = re.search(r"if \(\*abort_flag\)[^;]*?for \(int \w+ = max\(0", body, re.S)
     assert drain is None, "the last copies are waited for only if a wait has given up already"
-    assert re.search(r"for \(int \w+ = max\(0, issued - \w+\); \w+ < issued; \+\+\w+\)\s*rla_mbar_wait\(&full", body)
+    assert re.search(r"for \(int \w+ = max\(0, (issued\w*) - \w+\); \w+ < \1; \+\+\w+\)\s*rla_mbar_wait\(&(?:sm\.)?full", body)
 
 
 def test_the_pair_drains_when_both_ctas_are_through():
