@@ -171,6 +171,15 @@ RLA_DEVFN uint32_t rla_cluster_nctarank() {
 RLA_DEVFN void rla_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of rla_cluster_sync.
+RLA_DEVFN void rla_cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+RLA_DEVFN void rla_cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // 16-byte load from CTA `rank`'s copy of the shared variable at `p`.
 RLA_DEVFN float4 rla_ld_dsmem_f4(const void* p, uint32_t rank) {
   uint32_t remote;

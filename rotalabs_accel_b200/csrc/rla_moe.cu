@@ -169,15 +169,6 @@ RLA_DEVFN float rla_ld_dsmem_f32(const void* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(rla_mapa(rla_smem_u32(p), rank)) : "memory");
   return v;
 }
-// The two halves of rla_cluster_sync.
-RLA_DEVFN void rla_cluster_arrive() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-RLA_DEVFN void rla_cluster_wait() {
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 RLA_DEVFN uint4 rla_lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));

@@ -31,10 +31,12 @@
 // Waits.  Every mbarrier wait is bounded; after one that gave up, the CTAs still
 // see all their copies land and their MMAs end before they leave.  The cluster's
 // barriers and tcgen05.alloc have no limit.  A barrier is reached by every
-// warp whatever its waits returned.  An allocation waits for CTAs of the same
-// SM to leave: this library's kernels cannot wait for one another in a circle
-// (see kW8PairSmem); a library's kernel on another stream that holds Tensor
-// Memory on one SM while it waits for another SM's is not excluded.
+// warp whatever its waits returned.  An allocation waits for other CTAs of its
+// SM to hand Tensor Memory back, and none of those waits for this one in turn:
+// a split CTA holds Tensor Memory only while it waits for its own copies and MMAs,
+// not for its cluster, and a CTA pair is alone on its SMs (kW8PairSmem).  Not
+// excluded: a kernel of another library, earlier in the stream, that lets
+// dependent kernels start before it has allocated its own.
 #include <algorithm>
 #include <atomic>
 
@@ -80,6 +82,10 @@ RLA_DEVFN void rla_tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&v)[16]) {
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
+}
+// Counted at the named barrier without waiting there.
+RLA_DEVFN void rla_named_bar_arrive(int id, int nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 RLA_DEVFN uint32_t rla_mapa(uint32_t addr, uint32_t rank) {
   uint32_t remote;
@@ -325,6 +331,9 @@ __global__ void __launch_bounds__(w8::THREADS, 5)
   rla_griddep_wait();  // before any read of what an earlier kernel may have written
 
   bool ok = true;
+  int* part = reinterpret_cast<int*>(ring);  // [bt][128], once every copy and MMA of the ring is done
+  const int cols = min(bt, out.M - m0);
+  const int t = threadIdx.x - 64;
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0;
@@ -370,8 +379,6 @@ __global__ void __launch_bounds__(w8::THREADS, 5)
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int n = n0 + row;
-    const int t = threadIdx.x - 64;
-    const int cols = min(bt, out.M - m0);
     for (int c = t; c < cols; c += 128) sx_s[c] = out.sx[m0 + c];
     const float sw = n < out.N ? w8a8_channel(out.sw, out.sw_f32 ? 2 : 1, n) : 0.f;
     const float bias = n < out.N ? w8a8_channel(out.bias, out.bias_kind, n) : 0.f;
@@ -381,7 +388,6 @@ __global__ void __launch_bounds__(w8::THREADS, 5)
     ok = rla_mbar_wait(&dfull, 0, RLA_DEVERR_TIMEOUT_ACCUM, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     rla_tc_fence_after();
-    int* part = reinterpret_cast<int*>(ring);  // [bt][128]: every copy and MMA of the ring is done
     if (ok && splits == 1) {
       w8a8_store_warp(out, tmem + lane_addr, 0, 32, cols, m0, n0 + quarter * 32, sw, bias, sx_s,
                       reinterpret_cast<__half*>(ring) + quarter * (32 * 32));
@@ -395,50 +401,57 @@ __global__ void __launch_bounds__(w8::THREADS, 5)
         for (int i = 0; i < 16; ++i) part[(j + i) * w8::BR + row] = static_cast<int>(d[i]);
       }
     }
-    if (splits > 1) {
-      __syncwarp();
-      rla_cluster_sync();
-      // thread t: four channels (16 bytes) of the columns rank + splits * (t / 32 + 4 i);
-      // all ranks' loads are issued before the first is used
-      if (ok) {
-        const int r4 = lane * 4;
-        const uint32_t mine = rla_smem_u32(part) + r4 * 4;
-        for (int c = rank + splits * (t >> 5); c < cols; c += splits * 4) {
-          int4 v[w8::MAX_SPLITS];
-#pragma unroll
-          for (int r = 0; r < w8::MAX_SPLITS; ++r)
-            if (r < splits) v[r] = rla_ld_cluster_int4(rla_mapa(mine + c * (w8::BR * 4), r));
-          int4 sum = v[0];
-#pragma unroll
-          for (int r = 1; r < w8::MAX_SPLITS; ++r)
-            if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
-          const float sx = sx_s[c];
-          const float4 w4 = *reinterpret_cast<const float4*>(sw_s + r4), b4 = *reinterpret_cast<const float4*>(bias_s + r4);
-          __half* yp = out.y + (int64_t)(m0 + c) * out.ldy + n0 + r4;
-          alignas(8) const __half h[4] = {w8a8_value(sum.x, w4.x, sx, b4.x), w8a8_value(sum.y, w4.y, sx, b4.y),
-                               w8a8_value(sum.z, w4.z, sx, b4.z), w8a8_value(sum.w, w4.w, sx, b4.w)};
-          if (out.vec >= 4 && n0 + r4 + 4 <= out.N) {
-            *reinterpret_cast<uint2*>(yp) = *reinterpret_cast<const uint2*>(h);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n0 + r4 + i < out.N) yp[i] = h[i];
-          }
-        }
-      }
-      __syncwarp();
-      rla_cluster_sync();  // nobody leaves while its shared memory may still be read
-    }
-  }
-  if (warp < 2 && splits > 1) {
-    rla_cluster_sync();
-    rla_cluster_sync();
   }
   rla_tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    rla_tc_fence_after();
-    rla_tmem_dealloc(tmem, tmem_cols);
+  if (splits == 1) {
+    __syncthreads();
+    if (warp == 1) {
+      rla_tc_fence_after();
+      rla_tmem_dealloc(tmem, tmem_cols);
+    }
+  } else {
+    // Tensor Memory goes back before the CTA waits for its cluster: holding it
+    // meanwhile, it could be what the cluster's other CTAs wait for (their
+    // allocation behind one of a third kernel that is stuck on these columns).
+    rla_cluster_arrive();
+    if (warp == 1) {
+      rla_named_bar_sync(2, 160);  // the epilogue warps have read it
+      rla_tc_fence_after();
+      rla_tmem_dealloc(tmem, tmem_cols);
+    } else if (warp >= 2) {
+      rla_named_bar_arrive(2, 160);
+    }
+    rla_cluster_wait();
+    // thread t: four channels (16 bytes) of the columns rank + splits * (t / 32 + 4 i);
+    // all ranks' loads are issued before the first is used
+    if (warp >= 2 && ok) {
+      const int r4 = lane * 4;
+      const uint32_t mine = rla_smem_u32(part) + r4 * 4;
+      for (int c = rank + splits * (t >> 5); c < cols; c += splits * 4) {
+        int4 v[w8::MAX_SPLITS];
+#pragma unroll
+        for (int r = 0; r < w8::MAX_SPLITS; ++r)
+          if (r < splits) v[r] = rla_ld_cluster_int4(rla_mapa(mine + c * (w8::BR * 4), r));
+        int4 sum = v[0];
+#pragma unroll
+        for (int r = 1; r < w8::MAX_SPLITS; ++r)
+          if (r < splits) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+        const float sx = sx_s[c];
+        const float4 w4 = *reinterpret_cast<const float4*>(sw_s + r4), b4 = *reinterpret_cast<const float4*>(bias_s + r4);
+        __half* yp = out.y + (int64_t)(m0 + c) * out.ldy + n0 + r4;
+        alignas(8) const __half h[4] = {w8a8_value(sum.x, w4.x, sx, b4.x), w8a8_value(sum.y, w4.y, sx, b4.y),
+                                        w8a8_value(sum.z, w4.z, sx, b4.z), w8a8_value(sum.w, w4.w, sx, b4.w)};
+        if (out.vec >= 4 && n0 + r4 + 4 <= out.N) {
+          *reinterpret_cast<uint2*>(yp) = *reinterpret_cast<const uint2*>(h);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n0 + r4 + i < out.N) yp[i] = h[i];
+        }
+      }
+    }
+    __syncwarp();
+    rla_cluster_sync();  // nobody leaves while its shared memory may still be read
   }
 }
 
@@ -684,10 +697,7 @@ struct W8Plan {
 
 // A pair CTA takes all of its SM's shared memory, although it needs less, so
 // that no other CTA with Tensor Memory sits beside it: a pair holds all 512
-// columns of one SM while it waits for those of the other, and a split cluster
-// of another stream could hold those and wait for the first.  (Split CTAs among
-// themselves cannot: clusters take at least 57 KB for 128 columns or 22 KB for
-// 32, so what fits an SM's shared memory fits its 512 columns.)
+// columns of one SM while it waits for those of the other.
 constexpr int kW8PairSmem = 227 * 1024;
 static_assert(sizeof(W8PairShared) + 1024 <= kW8PairSmem, "the ring fits");
 
