@@ -7,7 +7,7 @@ rotalabs-accel has no mixture-of-experts layer.  On CUDA tensors the whole
 layer -- router, choice, gate/up, SwiGLU, down, combination -- is two kernels
 (``rla_moe``) for up to 32 tokens; longer batches run 32 tokens at a time.
 CPU tensors follow the same formulas in torch operations.  For inference: no
-gradients flow.
+gradients flow through ``int8_moe``, on either.
 """
 
 from __future__ import annotations
@@ -79,7 +79,9 @@ def int8_moe(x: torch.Tensor, router_weight: torch.Tensor, w_gate: torch.Tensor,
         y = _capi.torch_ops().moe(_as_2d_fp16(x, x.shape[-1]), router_weight, w_gate, scale_gate, w_up, scale_up,
                                   w_down, scale_down, top_k, renormalize)
         return y.view(x.shape)
-    return int8_moe_torch(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k, renormalize)
+    with torch.no_grad():
+        return int8_moe_torch(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k,
+                              renormalize)
 
 
 def _moe_args(x, router_weight, w_gate, scale_gate, w_up, scale_up, w_down, scale_down, top_k):

@@ -20,7 +20,9 @@ these join are ``rmsnorm`` (kernels/normalization.py:186-213), ``swiglu_fused``
 ``scale = max|v| / 127``, a zero row gets scale 1, round half to even.
 
 CUDA tensors run the sm_100a kernels (fp16 or bf16 activations); CPU tensors
-the same formulas in torch operations.  For inference: no gradients flow.
+the same formulas in torch operations (fp32 activations too, which the kernels
+refuse: a residual stream would lose bits in a cast).  For inference: no
+gradients flow, on either.
 """
 
 from __future__ import annotations
@@ -103,8 +105,9 @@ def add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch
     if x.is_cuda:
         y, h = _capi.torch_ops().add_rmsnorm(_rows(x), _rows(residual), weight, eps)
         return y.view(x.shape), x if residual is None else h.view(x.shape)
-    v, h = _norm_torch(x, residual, weight, eps)
-    return v.to(x.dtype), h
+    with torch.no_grad():
+        v, h = _norm_torch(x, residual, weight, eps)
+        return v.to(x.dtype), h
 
 
 def add_rmsnorm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6):
@@ -123,9 +126,10 @@ def add_rmsnorm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
     if x.is_cuda:
         q, s, h = _capi.torch_ops().add_rmsnorm_int8(_rows(x), _rows(residual), weight, eps)
         return q.view(x.shape), s.view(x.shape[:-1]), x if residual is None else h.view(x.shape)
-    v, h = _norm_torch(x, residual, weight, eps)
-    q, s = _quantize_rows(v)
-    return q, s, h
+    with torch.no_grad():
+        v, h = _norm_torch(x, residual, weight, eps)
+        q, s = _quantize_rows(v)
+        return q, s, h
 
 
 def swiglu_int8(gate: torch.Tensor, up: torch.Tensor):
@@ -141,7 +145,8 @@ def swiglu_int8(gate: torch.Tensor, up: torch.Tensor):
     if gate.is_cuda:
         q, s = _capi.torch_ops().swiglu_int8(_rows(gate), _rows(up))
         return q.view(gate.shape), s.view(gate.shape[:-1])
-    return _quantize_rows(_silu_mul(gate, up))
+    with torch.no_grad():
+        return _quantize_rows(_silu_mul(gate, up))
 
 
 def int8_gemm_w8a8(x_int8: torch.Tensor, x_scale: torch.Tensor, weight_int8: torch.Tensor, scale: torch.Tensor,
@@ -163,6 +168,7 @@ def int8_gemm_w8a8(x_int8: torch.Tensor, x_scale: torch.Tensor, weight_int8: tor
     if x_int8.is_cuda:
         y = _capi.torch_ops().w8a8_gemm(_rows(x_int8), x_scale.reshape(x_scale.numel()), weight_int8, scale, bias)
         return y.view(*x_int8.shape[:-1], weight_int8.shape[0])
-    # products of int8 summed in fp64: exact, as on the GPU
-    y = (x_int8.double() @ weight_int8.double().t()).float() * scale.float() * x_scale.unsqueeze(-1)
-    return (y if bias is None else y + bias.float()).half()
+    with torch.no_grad():
+        # products of int8 summed in fp64: exact, as on the GPU
+        y = (x_int8.double() @ weight_int8.double().t()).float() * scale.float() * x_scale.unsqueeze(-1)
+        return (y if bias is None else y + bias.float()).half()
