@@ -89,15 +89,15 @@ RLA_DEVFN __half rla_swiglu(float gate, float up) {
   return __float2half_rn(__fdividef(gu.x, 1.0f + __expf(-gu.x)) * gu.y);
 }
 
-// silu(f) * u in fp32 where f <= -87: 1 + e^-f is beyond the range of the
-// quotients above, and silu(f) = f e^f (to 2^-125) itself below fp32's, but a
-// large u brings the product back: -88 times 1e38 is -53.  So e^f is taken as the
-// square of e^(f / 2), one factor on each side of u.
-RLA_DEVFN float rla_silu_mul_far(float f, float u) {
-  const float t = f * 0.72134752f;  // log2(e) / 2
-  float h;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(h) : "f"(t));
-  return f * h * u * h;
+// silu(f) * u in fp32 for all f.  Below -87, 1 + e^-f is beyond the range of the
+// quotients above and silu(f) = f e^f soon below fp32's, but a large u brings the
+// product back: f = -88, u = 1e38 make -53.  So with t = e^(-|f| / 2) the quotient is by 1 + t^2,
+// and f < 0 has t as a factor on each side of u.
+RLA_DEVFN float rla_silu_mul(float f, float u) {
+  float t;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(f) * -0.72134752f));  // log2(e) / 2
+  const float h = f < 0.f ? t : 1.f;
+  return __fdividef(f * h, fmaf(t, t, 1.f)) * u * h;
 }
 
 // ---------------------------------------------------------------------------

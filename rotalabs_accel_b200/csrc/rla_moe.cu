@@ -4,8 +4,8 @@
 //      a = silu(sg * (Wg x)) * su * (Wu x) for every chosen expert
 //   2. down + combine:   y = fp16( sum over the chosen experts of
 //                                  c * sd * (Wd a) ),  c = p or p / sum p
-// a is the sum of two bf16 terms, a = hi + lo with hi = bf16(a), lo = bf16(a -
-// hi): 2^-16 of a at most is lost and fp32's range is kept (a may be far above
+// a is the sum of two bf16 terms, a = hi + lo with hi = a cut off to bf16, lo =
+// bf16(a - hi): 2^-16 of a at most is lost and fp32's range is kept (a may be far above
 // fp16's 65504 and the scales bring y back).  Tensor-core operands hold no more
 // bits, so the down product is Wd hi + Wd lo in one fp32 sum.
 //
@@ -35,7 +35,8 @@
 // (4096 x 2048) 75 -> 84.
 // A column with no token repeats another one's activations and is
 // dropped: columns of a product do not mix, and loads without conditions
-// keep the instructions of a 1 KB piece near the 40 of its conversion.
+// keep the instructions of a 1 KB piece near those of its conversion (40, and
+// 56 to bf16).
 //
 // Routing.  Which weights to read is not known before the logits are, so
 // the whole GPU waits for them.  Each cluster of 4 CTAs computes all logits by
@@ -143,11 +144,10 @@ RLA_DEVFN void rla_mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint3
 }
 // Where channel i lies in a row of `a`: the order of the conversion above.
 RLA_DEVFN int moe_place(int i) { return (i & ~3) | (i & 1) << 1 | (i >> 1 & 1); }
-// v = hi + lo.  (The largest finite values would round up to infinity; lo is 0
-// where v is infinite or NaN.)
+// v = hi + lo; hi is v cut off (the largest finite values would round up to
+// infinity), lo is 0 where v is infinite or NaN.
 RLA_DEVFN void moe_split(float v, __nv_bfloat16& hi, __nv_bfloat16& lo) {
-  hi = __float2bfloat16_rn(v);
-  if (fabsf(__bfloat162float(hi)) == INFINITY) hi = __float2bfloat16_rz(v);
+  hi = __float2bfloat16_rz(v);
   const float h = __bfloat162float(hi);
   lo = __float2bfloat16_rn(fabsf(h) < INFINITY ? v - h : 0.f);
 }
@@ -655,8 +655,7 @@ RLA_DEVFN void moe_finish_unit(const MoeArgs& g, const MoeRoute& r, int e, int g
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           const float gate = acc[m][t][j] * sc.gate[m], up = acc[m][t][2 + j] * sc.up[m];
-          const float a = gate < -87.f ? rla_silu_mul_far(gate, up) : __fdividef(gate, 1.0f + __expf(-gate)) * up;
-          moe_split(a, to[m * 8], to[g.I + m * 8]);
+          moe_split(rla_silu_mul(gate, up), to[m * 8], to[g.I + m * 8]);
         }
       }
     }

@@ -133,7 +133,7 @@ RLA_DEVFN void rows_swiglu_far(const RowVec<T, V>& a, const RowVec<T, V>& b, flo
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const float f = rows_to_f(a.v[i]);
-    if (f < -87.f) p[i] = rla_silu_mul_far(f, rows_to_f(b.v[i]));
+    if (f < -87.f) p[i] = rla_silu_mul(f, rows_to_f(b.v[i]));
     top = rows_max_nan(top, fabsf(p[i]));
   }
 }
@@ -502,9 +502,9 @@ static cudaError_t launch_rows_width(const RowsArgs& g, int op, cudaStream_t s) 
   const bool many = g.M >= 4 * device_sm_count();
   if constexpr (V == 8) {
     // CTAs an SM, threads and stages by measurement: 2048 x 4096 int8 14.0 us
-    // with three CTAs, 16.6 with two; 4096 x 8192 bf16 60 us without the
+    // with three CTAs, 16.6 with two; 4096 x 8192 bf16 to int8 60 us without the
     // stream, 40.7 with it (0.88 of the memory's rate); 4096 x 16384 119 and
-    // 79 us (0.91).  Not below 2048: 4096 x 1024 9.1 us without, 10.0 with it.
+    // 79 us (0.91); with a bf16 output 50.3 and 97.5 us.  Not below 2048: 4096 x 1024 9.1 us without, 10.0 with it.
     if (many && g.K >= 2048) {
       if (g.K <= 4096) return launch_rows_stream_cfg<T, 2, 256, 3, true>(g, op, s);
       if (g.K <= 8192) return launch_rows_stream_cfg<T, 4, 256, 2, true>(g, op, s);
