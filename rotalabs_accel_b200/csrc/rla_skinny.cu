@@ -159,9 +159,10 @@ RLA_DEVFN void skinny_body(const __half* __restrict__ x, int64_t ldx, const int8
   const uint4 zero4 = make_uint4(0, 0, 0, 0);
   // XJIT: each chunk's activation fragments are loaded just before its MMAs
   // instead of with the batch's weight loads, so that all the weight loads
-  // issue first.  Chosen per launch shape (XJ) from measurements, and always for
-  // one tile and 128 threads; the gated and exchange forms keep the batch order.
-  constexpr bool XJIT = XJ && !PEER && !GLU;
+  // issue first.  Chosen per launch shape (XJ) from measurements, and always
+  // for one tile and 128 threads and for four tiles gated; the other gated and
+  // the exchange forms keep the batch order.
+  constexpr bool XJIT = XJ && !PEER && (!GLU || NT == 4);
   for (int c = c_begin + wk; c < c_end; c += WK * U) {
     uint4 wa[U][2];
     XFrag<NT> xb[U];
@@ -421,11 +422,11 @@ __global__ void __launch_bounds__(32 * WN * WK) w8a16_skinny_kernel(RLA_SKINNY_P
 //  - one tile, 128 threads, B = 7 (72 registers).  Left to itself the exchange
 //    form gets 56, too few to keep a whole batch of loads in flight (one GPU,
 //    world-1 exchange, 8192 -> 14336 at M = 1: 28.7 -> 24.6 us), the plain form
-//    74, one CTA fewer (28672 -> 8192 at M = 1: 45 us, 61 with six CTAs).  The
-//    plain form also takes the XJIT order: its x loads are coherent, so the
-//    compiler does not move them behind the weights' itself, and a whole
-//    batch of both does not fit;
+//    74, one CTA fewer (28672 -> 8192 at M = 1: 45 us, 61 with six CTAs);
 //  - four tiles, gated: 80 registers, 86 without the bound (one CTA fewer).
+// Both take the XJIT order: x loads are coherent, so the compiler does not move
+// them behind the weights' itself, and a whole batch of both does not fit (gated
+// 4096 -> 11008 at M = 32: 42.6 us, 48.4 in the batch order).
 template <int NT, int WN, int WK, int U, bool PEER, bool GLU, bool XJ, int B>
 __global__ void __launch_bounds__(32 * WN * WK, B) w8a16_skinny_kernel_b(RLA_SKINNY_PARAMS) {
   skinny_body<NT, WN, WK, U, PEER, GLU, XJ>(RLA_SKINNY_ARGS);
@@ -469,15 +470,21 @@ struct SkinnyInst {
       return w8a16_skinny16_kernel<NT, U, XJ>;
     } else {
       if (form == 2) {
-        if constexpr (NT == 1 && WN * WK == 4) return w8a16_skinny_kernel_b<NT, WN, WK, U, true, false, XJ, 7>;
-        return w8a16_skinny_kernel<NT, WN, WK, U, true, false, XJ>;
+        if constexpr (NT == 1 && WN * WK == 4)
+          return w8a16_skinny_kernel_b<NT, WN, WK, U, true, false, XJ, 7>;
+        else
+          return w8a16_skinny_kernel<NT, WN, WK, U, true, false, XJ>;
       }
       if (form == 1) {
-        if constexpr (NT == 4) return w8a16_skinny_kernel_b<NT, WN, WK, U, false, true, XJ, 24 / (WN * WK)>;
-        return w8a16_skinny_kernel<NT, WN, WK, U, false, true, XJ>;
+        if constexpr (NT == 4)
+          return w8a16_skinny_kernel_b<NT, WN, WK, U, false, true, true, 24 / (WN * WK)>;
+        else
+          return w8a16_skinny_kernel<NT, WN, WK, U, false, true, XJ>;
       }
-      if constexpr (NT == 1 && WN * WK == 4) return w8a16_skinny_kernel_b<NT, WN, WK, U, false, false, true, 7>;
-      return w8a16_skinny_kernel<NT, WN, WK, U, false, false, XJ>;
+      if constexpr (NT == 1 && WN * WK == 4)
+        return w8a16_skinny_kernel_b<NT, WN, WK, U, false, false, true, 7>;
+      else
+        return w8a16_skinny_kernel<NT, WN, WK, U, false, false, XJ>;
     }
   }
   // CTAs that can be resident on the whole device at once when the K slices
