@@ -5,7 +5,8 @@ reference's ``SwiGLU``, src/rotalabs_accel/kernels/activations.py:140-181, over
 ``Int8Linear``, kernels/gemm.py:241-336), the weights of all experts stacked.
 rotalabs-accel has no mixture-of-experts layer.  On CUDA tensors the whole
 layer -- router, choice, gate/up, SwiGLU, down, combination -- is two kernels
-(``rla_moe``) for up to 32 tokens; longer batches run 32 tokens at a time.
+(``rla_moe``) for up to 32 tokens; longer batches run 32 tokens at a time and
+read their experts each time (256 tokens take eight times as long as 32).
 CPU tensors follow the same formulas in torch operations.  For inference: no
 gradients flow through ``int8_moe``, on either.
 """
